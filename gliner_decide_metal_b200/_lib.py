@@ -21,7 +21,7 @@ STATUS_NAMES = {
     8: "GDC_ERR_OUT_OF_MEMORY", 9: "GDC_ERR_TIMEOUT", 10: "GDC_ERR_UNSUPPORTED", 11: "GDC_ERR_NULL_POINTER",
     12: "GDC_ERR_PARTIAL",
 }
-GDC_INT32, GDC_INT64, GDC_FLOAT16, GDC_FLOAT32, GDC_UINT8 = range(5)
+GDC_INT32, GDC_INT64, GDC_FLOAT16, GDC_FLOAT32, GDC_UINT8, GDC_BFLOAT16 = range(6)
 
 
 class GdcConfig(C.Structure):
@@ -81,6 +81,13 @@ SIGNATURES = [
     ("gdc_disentangled_attention_scalar", C.c_int, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp]),
     ("gdc_disentangled_attention_noalloc", C.c_int, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp]),
     ("gdc_linear", C.c_int, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i64, _i32, _vp]),
+    ("gdc_packed_attention_workspace", C.c_int, [_i32, _i64, _i64, _i32, _i32, _i32, C.POINTER(C.c_size_t)]),
+    ("gdc_packed_attention", C.c_int, [C.c_int, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i32, _i64, _i64,
+                                       _i32, _i32, _i32, _i32, _f32, _vp, C.c_size_t, _vp]),
+    ("gdc_linear_residual", C.c_int, [C.c_int, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _vp, _i32, _i32,
+                                      _i32, _vp]),
+    ("gdc_gated_residual_norm", C.c_int, [C.c_int, _vp, _i64, _vp, _i64, _i32, _vp, _vp, _vp, _i64, _vp, _f32, _i32, _vp,
+                                          _vp, _vp, _i64, _vp, _i64, _i64, _vp, _i32, _f32, _vp]),
     ("gdc_kernels_check_errors", C.c_int, []),
     ("gdc_selftest_wait_timeout", C.c_int, [_i32, _vp]),
     ("gdc_last_error", C.c_char_p, []),

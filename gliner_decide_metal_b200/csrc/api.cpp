@@ -28,21 +28,6 @@ thread_local std::string g_last_error;
 std::mutex g_err_mu;
 int* g_err_words[64] = {};
 
-gdc_status device_error_word(int** out) {
-  int dev = 0;
-  GDC_CUDA_TRY(cudaGetDevice(&dev));
-  if (dev < 0 || dev >= 64) return set_error(GDC_ERR_CUDA, "device ordinal out of range");
-  std::lock_guard<std::mutex> lk(g_err_mu);
-  if (!g_err_words[dev]) {
-    int* p = nullptr;
-    GDC_CUDA_TRY(cudaMalloc(&p, 256));
-    GDC_CUDA_TRY(cudaMemset(p, 0, 256));
-    g_err_words[dev] = p;
-  }
-  *out = g_err_words[dev];
-  return GDC_OK;
-}
-
 size_t dtype_bytes(gdc_dtype d) {
   switch (d) {
     case GDC_INT32:
@@ -54,6 +39,8 @@ size_t dtype_bytes(gdc_dtype d) {
       return 2;
     case GDC_UINT8:
       return 1;
+    default:  // a type of the block operators only
+      return 0;
   }
   return 0;
 }
@@ -71,6 +58,8 @@ double read_value(const void* p, gdc_dtype d, int64_t i) {
       return double(static_cast<const float*>(p)[i]);
     case GDC_UINT8:
       return double(static_cast<const uint8_t*>(p)[i]);
+    default:
+      break;
   }
   return 0.0;
 }
@@ -205,6 +194,21 @@ gdc_status ensure_pinned(uint8_t** p, size_t* cap, size_t bytes) {
 }
 
 }  // namespace
+
+gdc_status device_error_word(int** out) {
+  int dev = 0;
+  GDC_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64) return set_error(GDC_ERR_CUDA, "device ordinal out of range");
+  std::lock_guard<std::mutex> lk(g_err_mu);
+  if (!g_err_words[dev]) {
+    int* p = nullptr;
+    GDC_CUDA_TRY(cudaMalloc(&p, 256));
+    GDC_CUDA_TRY(cudaMemset(p, 0, 256));
+    g_err_words[dev] = p;
+  }
+  *out = g_err_words[dev];
+  return GDC_OK;
+}
 
 gdc_status set_error(gdc_status st, const char* fmt, ...) {
   char buf[1024];
@@ -719,6 +723,9 @@ gdc_status gdc_kernels_check_errors(void) {
   if (h != 0) {
     GDC_CUDA_TRY(cudaMemset(err, 0, sizeof(int)));
     if (h & kErrTimeout) return set_error(GDC_ERR_TIMEOUT, "a device-side wait exceeded its time limit");
+    if (h & kErrBadOffsets)
+      return set_error(GDC_ERR_INVALID_INPUT, "packed offsets decrease or leave the buffers' rows");
+    if (h & kErrBadGateIndex) return set_error(GDC_ERR_INVALID_INPUT, "a gate index is outside [0, gate_rows)");
     return set_error(GDC_ERR_CUDA, "device error word 0x%x", h);
   }
   return GDC_OK;

@@ -60,7 +60,13 @@ enum DeviceErrorBits : int {
   kErrTimeout = 1,          // an mbarrier / flag wait exceeded its limit
   kErrBadTokenId = 2,       // input id outside [0, vocab)
   kErrBadMarkerIndex = 4,   // marker index outside [0, seq_len)
+  kErrBadOffsets = 8,       // packed offsets that decrease or leave the buffers' rows
+  kErrBadGateIndex = 16,    // gate index outside [0, gate_rows)
 };
+
+// The current device's error word of the kernel-level entry points (no model handle);
+// allocated by the first call on a device.
+gdc_status device_error_word(int** out);
 
 // fp16 <-> fp32 on the host (IEEE binary16, round-to-nearest-even).
 uint16_t f32_to_f16_bits(float f);

@@ -101,6 +101,48 @@ gdc_status launch_classifier_out(const __half* h, const __half* w2, const __half
 gdc_status launch_decode(const float* logits, int batch, int max_heads, int max_options, const int32_t* n_labels,
                          const uint8_t* multi_label, float* probs, uint8_t* selected, cudaStream_t stream);
 
+// ---- block operators over packed rows (arguments already checked by block_api.cpp) ----
+
+// Element type of a block operator's tensors.
+enum class Elem : int { kF16 = 0, kBF16 = 1 };
+
+// Activation of the linear epilogue beyond Act's three.
+constexpr int kActSilu = 3;
+
+struct PackedAttentionArgs {
+  const void *q, *k, *v;
+  void* out;
+  int64_t ldq, ldk, ldv, ldo;
+  const int32_t *q_off, *k_off;
+  int batch;
+  int64_t q_rows, k_rows;
+  int heads, kv_heads, dim;
+  bool causal;
+  float scale;
+  uint8_t* workspace;
+};
+size_t packed_attention_workspace(int batch, int64_t q_rows, int64_t k_rows, int heads, int kv_heads, int dim);
+gdc_status launch_packed_attention(Elem t, const PackedAttentionArgs& a, cudaStream_t stream, int* err);
+
+struct LinearResidualArgs {
+  const void *a, *w, *bias, *residual;
+  void* out;
+  int64_t lda, ldw, ldr, ldo, M;
+  const int32_t* rows_dev;
+  int N, K, act;
+};
+gdc_status launch_linear_residual(Elem t, const LinearResidualArgs& a, cudaStream_t stream, int* err);
+
+struct GatedNormArgs {
+  const void *y, *x, *post_w, *post_b, *gate, *pre_w, *pre_b;
+  void *x_out, *n_out;
+  int64_t ldy, ldx, ldxo, ldno, rows, gate_rows;
+  const int32_t *gate_index, *rows_dev;
+  int post, pre, cols;  // norm kinds: 0 none, 1 LayerNorm, 2 RMSNorm
+  float scale, eps;
+};
+gdc_status launch_gated_residual_norm(Elem t, const GatedNormArgs& a, cudaStream_t stream, int* err);
+
 int device_sm_count(int device);
 
 // Failure-detection self-test: a kernel whose bounded wait on an mbarrier that never

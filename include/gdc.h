@@ -54,7 +54,8 @@ typedef enum gdc_dtype {
   GDC_INT64 = 1,
   GDC_FLOAT16 = 2,
   GDC_FLOAT32 = 3,
-  GDC_UINT8 = 4
+  GDC_UINT8 = 4,
+  GDC_BFLOAT16 = 5 /* block operators only (gdc_packed_attention and the two after it) */
 } gdc_dtype;
 
 /* DeBERTaV2Configuration (Configuration.swift:3-49) plus the init flags of
@@ -320,8 +321,86 @@ gdc_status gdc_disentangled_attention_noalloc(const uint16_t* qkv, const uint16_
 gdc_status gdc_linear(const uint16_t* a, const uint16_t* w, const uint16_t* bias, uint16_t* out,
                       int64_t M, int32_t N, int32_t K, int64_t ldo, int32_t act, void* stream);
 
+/* ---- Block operators over packed rows (device pointers; enqueued on `stream`). ----
+ * The three operators of a transformer block whose rows are the tokens of sequences of
+ * different lengths laid back to back, next to the three above; they have no counterpart in
+ * the reference. Common rules:
+ *  - dtype is GDC_FLOAT16 or GDC_BFLOAT16, the type of every tensor of the call; sums, softmax
+ *    statistics and norms are held in 32 bits and results rounded once.
+ *  - All pointers are memory of the current device, and `stream` (NULL = the default stream) is
+ *    a stream of it. Nothing synchronises or allocates, except that the first call on a device
+ *    sets up the error word of gdc_kernels_check_errors: make that call before any stream
+ *    capture. A captured call may be replayed with new contents of every tensor, offsets,
+ *    indices and row counts included.
+ *  - What only the device can see (offsets, indices) is checked there: a bad value is skipped
+ *    as described below, never followed out of range, and the next gdc_kernels_check_errors()
+ *    returns GDC_ERR_INVALID_INPUT.
+ *  - rows_dev (may be NULL): a device int32, read when the call runs; only rows
+ *    [0, min(rows, *rows_dev)) are computed and written, rows behind them stay as they were. With
+ *    packed sequences this is the last entry of the offsets.
+ *  - Outputs must not overlap inputs, except where said. */
+
+/* Softmax attention with grouped heads over packed sequences. Sequence b has the query rows
+ * [q_off[b], q_off[b+1]) of q and out and the key rows [k_off[b], k_off[b+1]) of k and v, Lq and
+ * Lk of them. Query i of Lq sees the keys j of its sequence with j <= i + Lk - Lq when causal
+ * (the queries are the sequence's last rows: all of them for a prompt, one for a sequence that
+ * takes one token at a time), every key otherwise; head h reads key / value head
+ * h / (heads / kv_heads):
+ *   out[i, h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * q[i, h] . k[j] - max)
+ * A query that sees no key gives zeros. What a query does not see never reaches its output, not
+ * even where it is infinite or NaN.
+ *  q, out: q_rows rows of heads * head_dim; k, v: k_rows rows of kv_heads * head_dim; row pitches
+ *  ldq, ldk, ldv, ldo in elements (q, k and v may be column blocks of one projection's output).
+ *  Pointers 16-byte aligned, pitches multiples of 8. head_dim is 64 or 128, heads a multiple of
+ *  kv_heads of at most 128 times it. scale is positive and finite.
+ *  q_off, k_off: device int32 [batch + 1]; k_off NULL means q_off. Rows outside every sequence are
+ *  neither read nor written. A sequence whose offsets decrease or leave [0, q_rows] or
+ *  [0, k_rows] is skipped (its rows stay as they were) and reported.
+ *  workspace: device memory of gdc_packed_attention_workspace() bytes for the same sizes, 256-byte
+ *  aligned, its contents arbitrary; calls that may run at the same time (graphs that share it
+ *  too) need one each. */
+gdc_status gdc_packed_attention_workspace(int32_t batch, int64_t q_rows, int64_t k_rows,
+                                          int32_t heads, int32_t kv_heads, int32_t head_dim,
+                                          size_t* bytes);
+gdc_status gdc_packed_attention(gdc_dtype dtype, const void* q, int64_t ldq, const void* k,
+                                int64_t ldk, const void* v, int64_t ldv, void* out, int64_t ldo,
+                                const int32_t* q_off, const int32_t* k_off, int32_t batch,
+                                int64_t q_rows, int64_t k_rows, int32_t heads, int32_t kv_heads,
+                                int32_t head_dim, int32_t causal, float scale, void* workspace,
+                                size_t workspace_bytes, void* stream);
+
+/* out[m, n] = residual[m, n] + act(sum_k a[m, k] w[n, k] + bias[n]), one rounding at the end;
+ * act: 0 = none, 1 = exact-erf GELU, 2 = ReLU, 3 = SiLU. Any M >= 0, N >= 1, K >= 1.
+ *  a [M, K] and w [N, K]: pointers 16-byte aligned, pitches multiples of 8 elements. bias [N] and
+ *  residual [M, N] may be NULL; they and out need only their type's alignment, any pitch >= N.
+ *  residual may be out itself (same pointer and pitch). */
+gdc_status gdc_linear_residual(gdc_dtype dtype, const void* a, int64_t lda, const void* w,
+                               int64_t ldw, const void* bias, const void* residual, int64_t ldr,
+                               void* out, int64_t ldo, int64_t M, const int32_t* rows_dev,
+                               int32_t N, int32_t K, int32_t act, void* stream);
+
+/* The norms before and after a block with its gate and residual scale, in one pass:
+ *   x_out = x + scale * gate * N_post(y)
+ *   n_out = N_pre(x_out before it is rounded)
+ * post_norm, pre_norm: 0 = none (post: N_post(y) = y; pre: no n_out, which is then NULL),
+ * 1 = LayerNorm, 2 = RMSNorm, each over a row's cols values with `eps` added to the (biased)
+ * variance or mean square, times weight, plus bias; NULL weight = 1, NULL bias = 0.
+ *  y NULL: no block before (x_out = x; x_out may then be NULL). x_out may be x itself (same pitch),
+ *  n_out may be y itself.
+ *  gate: [gate_rows, cols], rows cols apart, or NULL (= 1). gate_index (device int32 [rows]) names
+ *  the gate row of every row; without it gate_rows is 1 (one row for all) or at least rows (one each).
+ *  A row whose index is outside [0, gate_rows) is skipped and reported.
+ *  cols in [1, 16384]; pitches in elements, at least cols; no alignment beyond the type's. */
+gdc_status gdc_gated_residual_norm(gdc_dtype dtype, const void* y, int64_t ldy, const void* x,
+                                   int64_t ldx, int32_t post_norm, const void* post_weight,
+                                   const void* post_bias, const void* gate, int64_t gate_rows,
+                                   const int32_t* gate_index, float scale, int32_t pre_norm,
+                                   const void* pre_weight, const void* pre_bias, void* x_out,
+                                   int64_t ldxo, void* n_out, int64_t ldno, int64_t rows,
+                                   const int32_t* rows_dev, int32_t cols, float eps, void* stream);
+
 /* Reads and clears the current device's error word used by the kernel-level entry
- * points above (bounded-wait timeouts). Synchronises the device. */
+ * points above (bounded-wait timeouts, bad offsets and indices). Synchronises the device. */
 gdc_status gdc_kernels_check_errors(void);
 
 /* Failure-detection self-test (no counterpart in the reference): launches a kernel whose
