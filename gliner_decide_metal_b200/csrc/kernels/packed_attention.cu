@@ -1,76 +1,975 @@
-// Softmax attention with grouped heads over packed sequences: one warp per query row and head,
-// online softmax in fp32 on CUDA cores.
+// Softmax attention with grouped heads over packed sequences on tcgen05 tensor cores.
+//
+//   s_ij = scale * q_i . k_j over the keys j that query i sees,
+//   o_i  = sum_j 2^(c s'_ij - c m_i) v_j / sum_j 2^(c s'_ij - c m_i),   s' = q.k, c = scale log2 e
+//
+// in one pass over the keys: a running reference m_i of the row's maximum and the running sum
+// stay in registers, the unnormalised o_i in TMEM.
+//
+// Rows. A query tile is 128 MMA rows: row r holds query position pos + r / G and head
+// hk * G + r % G of key head hk (G = heads / kv_heads), so a key / value tile is read once for
+// all heads of its group and a single token's G heads fill one tile. One work item is two such
+// tiles (256 rows) of one sequence and key head against a range of 128-key tiles.
+//
+// Roles of a CTA (one per SM, persistent over items):
+//   warps 0-3, 4-7  softmax of tile 0 / tile 1: one thread a row. Reads its 128 scores from TMEM,
+//                   writes the weights back over them as 16-bit MMA operands, and at an item's
+//                   end divides and stores the row (or stores the split's partial row).
+//   warp 8          issues the MMAs: S_t = Q_t K_j^T (both operands in shared memory), then
+//                   O_t += P_t V_j (P_t from TMEM); the tensor cores work on one tile while the
+//                   softmax warps work on the other.
+//   warp 9          TMA: Q tiles of the item and a ring of K and V tiles, running ahead into the
+//                   next item.
+// TMEM: S_0 [0, 128), S_1 [128, 256), O_0 [256, 256 + D), O_1 behind it; P_t lies over S_t.
+//
+// The reference m_i moves only when a row's maximum has grown by more than 2^8 (then the tile's
+// O rows are rescaled in TMEM): weights stay below 2^8, which 16-bit weights and fp32 sums hold
+// without loss, and most key tiles need no rescale. S_t(j) complete implies P_t V(j-1) complete
+// (one thread issues them in that order), so the rescale needs no wait of its own.
+//
+// A value that no visible key contributes must not reach a row, but 0 * inf is NaN: a row whose
+// result is not finite is computed again from memory by one warp over exactly its visible keys
+// (row_by_definition); value rows behind the last key of a sequence are zeroed in shared memory
+// first, so ordinary padding never takes that path.
+//
+// Plan. Lengths are device data. When there are more items than SMs, or few items with many keys,
+// plan_kernel lists the items, splits long key ranges into chunks (their partial rows are joined
+// by combine_kernel), and orders them by descending cost; otherwise a CTA finds its item itself.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+
 #include "elem.cuh"
 #include "kernels.h"
 #include "ptx.cuh"
 
 namespace gdc {
+
+PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn();
+
 namespace {
 
-// Index of the sequence that holds `row`: the last b with off[b] <= row among those whose rows
-// [off[b], off[b+1]) are valid. -1: none.
-__device__ __forceinline__ int find_sequence(const int32_t* off, int batch, int row) {
-  for (int b = 0; b < batch; ++b)
-    if (off[b] <= row && row < off[b + 1]) return b;
-  return -1;
+constexpr int kKeys = 128;       // keys of a tile
+constexpr int kThreads = 384;     // three warpgroups; two of the third's warps only take part in barriers
+constexpr int kRowRegs = 216, kIssueRegs = 72;  // 256 * 216 + 128 * 72 = 384 * 168, the launch's registers
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanSms = 148;    // the planner's unit of work (the workspace size depends on it)
+constexpr float kGrowth = 8.0f;  // log2 growth of a row's maximum that moves its reference
+
+// One work item (32 bytes).
+struct Item {
+  int q_row, lq;   // first query row and number of queries of the sequence
+  int k_row, lk;   // first key row and number of keys
+  int pos;         // first query position of the item
+  int t0, t1;      // key tiles [t0, t1)
+  int slot;        // partial rows' slot, -1: the item's only range
+};
+struct SplitItem {  // an item whose key range was split: slots [slot, slot + n)
+  int q_row, lq, k_row, lk, pos, slot, n, pad;
+};
+struct PlanHeader {
+  int n_items, n_splits;
+};
+
+// Workspace: header, items, split items, partial rows (fp32 O, then reference and sum).
+struct PlanLayout {
+  int64_t items_ub;    // upper bound of (sequence, item) pairs
+  int rows_cap;        // rows of an item that can be used
+  int chunks_cap;      // planned items per key head, splits included
+  bool planned, split;
+  size_t items_at, splits_at, part_o_at, part_ml_at, bytes;
+};
+
+PlanLayout plan_layout(int batch, int64_t q_rows, int64_t k_rows, int heads, int kv_heads, int dim) {
+  PlanLayout l{};
+  const int G = heads / kv_heads;
+  const int per_item = 2 * (kKeys / G);
+  l.items_ub = q_rows / per_item + std::min<int64_t>(batch, q_rows);
+  l.rows_cap = int(std::min<int64_t>(int64_t(per_item) * G, q_rows * G));
+  const int64_t jobs = l.items_ub * kv_heads;
+  // Splitting pays while there are few jobs to an SM; partial rows are bounded to 64 MB.
+  const int64_t row_bytes = int64_t(l.rows_cap) * (dim + 2) * 4;
+  const int64_t cap = std::min<int64_t>((int64_t(64) << 20) / row_bytes, jobs + 8 * kPlanSms);
+  l.split = k_rows > 2 * kKeys && jobs <= 8 * kPlanSms && cap >= jobs + kPlanSms / 2;
+  l.planned = l.split || jobs > kPlanSms;
+  l.chunks_cap = int(l.split ? cap / kv_heads : std::min<int64_t>(l.items_ub, INT32_MAX));
+  auto up = [](size_t v) { return (v + 255) & ~size_t(255); };
+  l.items_at = 256;
+  l.splits_at = l.items_at + (l.planned ? up(size_t(l.chunks_cap) * sizeof(Item)) : 0);
+  l.part_o_at = l.splits_at + (l.split ? up(size_t(l.items_ub) * sizeof(SplitItem)) : 0);
+  l.part_ml_at = l.part_o_at + (l.split ? up(size_t(l.chunks_cap) * kv_heads * l.rows_cap * dim * 4) : 0);
+  l.bytes = l.part_ml_at + (l.split ? up(size_t(l.chunks_cap) * kv_heads * l.rows_cap * 8) : 0);
+  return l;
 }
 
+struct Params {
+  const void *q, *k, *v;
+  void* out;
+  long long ldq, ldk, ldv, ldo;
+  const int32_t *q_off, *k_off;
+  int batch, q_rows, k_rows, heads, kv_heads, group, tile_pos;  // tile_pos: positions of a tile
+  int causal;
+  float scale, scale_log2;
+  // plan
+  PlanHeader* header;
+  Item* items;
+  SplitItem* splits;
+  float* part_o;   // [slot * kv_heads + hk][rows_cap][D]
+  float2* part_ml; // [slot * kv_heads + hk][rows_cap]
+  int rows_cap, chunks_cap, splits_cap;
+  int can_split;
+  int* err;
+};
+
+// Offsets of sequence b; false (and reported by `lane`) where they are not those of the buffers.
+__device__ __forceinline__ bool sequence(const Params& p, int b, bool report, int& q0, int& lq, int& k0, int& lk) {
+  q0 = p.q_off[b];
+  const int q1 = p.q_off[b + 1];
+  k0 = p.k_off[b];
+  const int k1 = p.k_off[b + 1];
+  lq = q1 - q0;
+  lk = k1 - k0;
+  const bool ok = q0 >= 0 && q1 >= q0 && q1 <= p.q_rows && k0 >= 0 && k1 >= k0 && k1 <= p.k_rows;
+  if (!ok && report) atomicOr(p.err, kErrBadOffsets);
+  return ok;
+}
+
+// Keys that query position `pos` sees (a prefix of the sequence's keys).
+__device__ __forceinline__ int seen_keys(int pos, int lq, int lk, int causal) {
+  return causal ? max(0, min(lk, pos + 1 + lk - lq)) : lk;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+
+// One output row from memory over exactly its visible keys: plain softmax in fp32, one warp.
+// The result is left in the lanes' o[D / 32] (columns lane * D / 32 ...).
 template <typename T, int D>
-__global__ void __launch_bounds__(128)
-    packed_attention_rows_kernel(PackedAttentionArgs a, int* err) {
+__device__ void row_by_definition(const Params& p, int q_row, int lq, int k_row, int lk, int pos, int head, float (&o)[D / 32]) {
   using E = ElemOps<T>;
   constexpr int PER = D / 32;
   const int lane = threadIdx.x & 31;
-  const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int row = int(item / a.heads), h = int(item % a.heads);
-  if (item < a.batch && lane == 0) {  // sequences without a row of their own are checked too
-    const int b = int(item);
-    if (a.q_off[b] > a.q_off[b + 1] || a.k_off[b] > a.k_off[b + 1]) atomicOr(err, kErrBadOffsets);
+  const int hk = head / p.group;
+  const T* q = static_cast<const T*>(p.q) + (long long)(q_row + pos) * p.ldq + head * D + lane * PER;
+  const T* k = static_cast<const T*>(p.k) + (long long)k_row * p.ldk + hk * D + lane * PER;
+  const T* v = static_cast<const T*>(p.v) + (long long)k_row * p.ldv + hk * D + lane * PER;
+  const int n = seen_keys(pos, lq, lk, p.causal);
+  float qv[PER], m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    qv[i] = E::to_f32(q[i]);
+    o[i] = 0.f;
   }
-  if (row >= a.q_rows) return;
-  const int b = find_sequence(a.q_off, a.batch, row);
-  if (b < 0) return;
-  const int q0 = a.q_off[b], q1 = a.q_off[b + 1], k0 = a.k_off[b], k1 = a.k_off[b + 1];
-  if (q0 < 0 || q1 > a.q_rows || k0 < 0 || k1 < k0 || k1 > a.k_rows) {
-    if (lane == 0) atomicOr(err, kErrBadOffsets);
-    return;
-  }
-  const int seen = a.causal ? max(0, min(k1 - k0, row - q1 + 1 + (k1 - k0))) : k1 - k0;
-  const T* q = static_cast<const T*>(a.q) + (long long)row * a.ldq + h * D + lane * PER;
-  const int hk = h / (a.heads / a.kv_heads);
-  const T* k = static_cast<const T*>(a.k) + (long long)k0 * a.ldk + hk * D + lane * PER;
-  const T* v = static_cast<const T*>(a.v) + (long long)k0 * a.ldv + hk * D + lane * PER;
-  float qv[PER], o[PER] = {}, m = -INFINITY, l = 0.f;
-  for (int i = 0; i < PER; ++i) qv[i] = E::to_f32(q[i]) * a.scale;
-  for (int j = 0; j < seen; ++j) {
+  for (int j = 0; j < n; ++j) {
     float s = 0.f;
-    for (int i = 0; i < PER; ++i) s = fmaf(qv[i], E::to_f32(k[(long long)j * a.ldk + i]), s);
-    s = ptx::warp_sum(s);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) s = fmaf(qv[i], E::to_f32(k[(long long)j * p.ldk + i]), s);
+    s = ptx::warp_sum(s) * p.scale;
     const float mn = fmaxf(m, s);
-    const float r = m == mn ? 1.f : expf(m - mn), p = expf(s - mn);
-    l = l * r + p;
-    for (int i = 0; i < PER; ++i) o[i] = o[i] * r + p * E::to_f32(v[(long long)j * a.ldv + i]);
+    const float r = m == mn ? 1.f : expf(m - mn), w = expf(s - mn);
+    l = l * r + w;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) o[i] = o[i] * r + w * E::to_f32(v[(long long)j * p.ldv + i]);
     m = mn;
   }
-  T* out = static_cast<T*>(a.out) + (long long)row * a.ldo + h * D + lane * PER;
-  for (int i = 0; i < PER; ++i) out[i] = E::from_f32(seen > 0 ? o[i] / l : 0.f);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) o[i] = n > 0 ? o[i] / l : 0.f;
+}
+
+template <typename T, int D>
+__device__ void store_row_by_definition(const Params& p, int q_row, int lq, int k_row, int lk, int pos, int head) {
+  using E = ElemOps<T>;
+  constexpr int PER = D / 32;
+  float o[PER];
+  row_by_definition<T, D>(p, q_row, lq, k_row, lk, pos, head, o);
+  uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + (long long)(q_row + pos) * p.ldo + head * D +
+                                              (threadIdx.x & 31) * PER);
+#pragma unroll
+  for (int i = 0; i < PER / 2; ++i) dst[i] = E::pack(o[2 * i], o[2 * i + 1]);
+}
+
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// ------------------------------------------------------------------------------------- plan
+
+constexpr int kBuckets = 512;
+
+// Lists the items by descending cost (key tiles of the chunk; a counting sort in shared memory)
+// and the split items. One CTA: a warp takes a sequence at a time, its lanes the items.
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(Params p) {
+  __shared__ int hist[kBuckets];
+  __shared__ unsigned long long s_work;
+  __shared__ int s_items, s_max, s_slots, s_splits;
+  pdl_launch();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = kPlanThreads / 32;
+  const int per_item = 2 * p.tile_pos;
+  if (threadIdx.x == 0) {
+    s_work = 0;
+    s_items = s_max = s_slots = s_splits = 0;
+  }
+  for (int i = threadIdx.x; i < kBuckets; i += kPlanThreads) hist[i] = 0;
+  __syncthreads();
+  auto tiles_of = [&](int pos, int lq, int lk) {
+    return (seen_keys(min(pos + per_item, lq) - 1, lq, lk, p.causal) + kKeys - 1) / kKeys;
+  };
+  {
+    unsigned long long work = 0;
+    int items = 0, most = 0;
+    for (int b = warp; b < p.batch; b += warps) {
+      int q0, lq, k0, lk;
+      if (!sequence(p, b, lane == 0, q0, lq, k0, lk)) continue;
+      const int n = (lq + per_item - 1) / per_item;
+      for (int i = lane; i < n; i += 32) {
+        const int t = tiles_of(i * per_item, lq, lk);
+        work += t;
+        ++items;
+        most = max(most, t);
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) work += __shfl_xor_sync(0xffffffffu, work, o);
+    items = __reduce_add_sync(0xffffffffu, items);
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0) {
+      atomicAdd(&s_work, work);
+      atomicAdd(&s_items, items);
+      atomicMax(&s_max, most);
+    }
+  }
+  __syncthreads();
+  // Chunk length. One round of chunks where the work allows short ones; otherwise about eight
+  // chunks an SM, none shorter than four tiles; at most chunks_cap chunks in all.
+  int chunk = 1 << 30;
+  if (p.can_split) {
+    const long long work = (long long)s_work * p.kv_heads, jobs = (long long)s_items * p.kv_heads;
+    auto ceil_div = [](long long a, long long b) { return (a + b - 1) / b; };
+    long long c = max(4ll, ceil_div(work, 8 * kPlanSms));
+    if (jobs <= kPlanSms / 2) {
+      const long long one = max(2ll, ceil_div(work, kPlanSms - jobs));
+      if (one <= 8) c = one;
+    }
+    const long long room = (long long)p.chunks_cap * p.kv_heads - jobs;
+    chunk = int(min((long long)chunk, max(c, ceil_div(work, max(1ll, room)))));
+  }
+  int shift = 0;
+  while ((min(chunk, s_max) >> shift) >= kBuckets) ++shift;
+  auto bucket = [&](int tiles) { return kBuckets - 1 - min(kBuckets - 1, tiles >> shift); };
+  for (int pass = 0; pass < 2; ++pass) {
+    for (int b = warp; b < p.batch; b += warps) {
+      int q0, lq, k0, lk;
+      if (!sequence(p, b, false, q0, lq, k0, lk)) continue;
+      const int n = (lq + per_item - 1) / per_item;
+      for (int i = lane; i < n; i += 32) {
+        const int t = tiles_of(i * per_item, lq, lk);
+        const int parts = t > chunk ? (t + chunk - 1) / chunk : 1;
+        const int len = (t + parts - 1) / parts;
+        int slot = -1;
+        if (pass == 1 && parts > 1) {
+          // (the bounds can only be met by overlapping sequences, which some bad offset, reported
+          // above, leaves behind; their items are then dropped)
+          slot = atomicAdd(&s_slots, parts);
+          if (slot + parts > p.chunks_cap) continue;
+          const int at = atomicAdd(&s_splits, 1);
+          if (at >= p.splits_cap) continue;
+          p.splits[at] = SplitItem{q0, lq, k0, lk, i * per_item, slot, parts, 0};
+        }
+        for (int c = 0; c < parts; ++c) {
+          const int t0 = min(t, c * len), t1 = min(t, t0 + len);
+          const int at = atomicAdd(&hist[bucket(t1 - t0)], 1);
+          if (pass == 1 && at < p.chunks_cap)
+            p.items[at] = Item{q0, lq, k0, lk, i * per_item, t0, t1, parts > 1 ? slot + c : -1};
+        }
+      }
+    }
+    __syncthreads();
+    if (pass == 0) {
+      // exclusive prefix sum of the histogram (descending cost: bucket 0 holds the longest)
+      int v = threadIdx.x < kBuckets ? hist[threadIdx.x] : 0;
+      int incl = v;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += u;
+      }
+      __shared__ int sums[32];
+      if (lane == 31) sums[warp] = incl;
+      __syncthreads();
+      int before = 0;
+      for (int w = 0; w < warp; ++w) before += sums[w];
+      if (threadIdx.x < kBuckets) hist[threadIdx.x] = before + incl - v;
+      __syncthreads();
+    }
+  }
+  if (threadIdx.x == 0) {
+    p.header->n_items = min(p.chunks_cap, hist[kBuckets - 1]);
+    p.header->n_splits = min(p.splits_cap, s_splits);
+  }
+}
+
+// ------------------------------------------------------------------------------------- main
+
+template <int D>
+struct Shape {
+  static constexpr int kAtoms = D / 64;
+  static constexpr int kTileBytes = 128 * D * 2;
+  static constexpr int kStages = D == 128 ? 5 : 10;
+  static constexpr int kOffQ = 0;
+  static constexpr int kOffRing = 2 * kTileBytes;
+  static constexpr int kOffBar = kOffRing + kStages * kTileBytes;
+  static constexpr int kSmemBytes = kOffBar + 512 + 1024;
+};
+
+struct Bars {
+  uint64_t full[10], empty[10];
+  uint64_t q_full[2], q_empty[2], s_full[2], p_ready[2], o_full[2], o_free[2], drain;
+  uint32_t tmem;
+  int item_ok;
+  Item item;
+};
+static_assert(sizeof(Bars) <= 512, "barrier block");
+
+__device__ __forceinline__ uint64_t desc_v(uint32_t addr) {
+  // MN-major, 128-byte swizzle: 64-column atoms 16 KB apart (leading offset), 8-key groups 1 KB
+  // apart (stride offset)
+  uint64_t d = uint64_t((addr >> 4) & 0x3FFFu);
+  d |= uint64_t(16384u >> 4) << 16;
+  d |= uint64_t(1024u >> 4) << 32;
+  d |= uint64_t(1u) << 46;
+  d |= uint64_t(2u) << 61;
+  return d;
+}
+
+// Key tiles of query tile `t` inside the item's range: [t0, t0 + n).
+__device__ __forceinline__ int tile_count(const Params& p, const Item& it, int t) {
+  const int first = it.pos + t * p.tile_pos;
+  if (first >= it.lq) return 0;
+  const int last = min(first + p.tile_pos, it.lq) - 1;
+  const int need = (seen_keys(last, it.lq, it.lk, p.causal) + kKeys - 1) / kKeys;
+  return max(0, min(it.t1, need) - it.t0);
+}
+
+// Walks a CTA's items: planned ones from the list, every other round backwards (the list is in
+// descending cost, so a CTA's share evens out); the unplanned one from shared memory.
+template <bool PLANNED>
+struct Walk {
+  const Params& p;
+  const Bars* bars;
+  long long jobs;
+  int round = 0;
+  __device__ Walk(const Params& p_, const Bars* b) : p(p_), bars(b) {
+    jobs = PLANNED ? (long long)p.header->n_items * p.kv_heads : 1;
+  }
+  __device__ __forceinline__ bool next(Item& it, int& hk) {
+    if (PLANNED) {
+      const long long g = gridDim.x;
+      const long long at = (long long)round * g + ((round & 1) ? g - 1 - blockIdx.x : blockIdx.x);
+      ++round;
+      if (at >= jobs) return false;  // only in the last round: earlier ones are full
+      const int4* src = reinterpret_cast<const int4*>(p.items + at / p.kv_heads);
+      const int4 a = src[0], b = src[1];
+      it = Item{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+      hk = int(at % p.kv_heads);
+      return true;
+    }
+    if (round++ > 0 || !bars->item_ok) return false;
+    it = bars->item;
+    hk = blockIdx.x % p.kv_heads;
+    return true;
+  }
+};
+
+template <typename T, int D, bool PLANNED>
+__global__ void __launch_bounds__(kThreads, 1)
+    packed_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                            const __grid_constant__ CUtensorMap tm_v, const Params p) {
+  using S = Shape<D>;
+  using E = ElemOps<T>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* s_q = smem + S::kOffQ;
+  uint8_t* s_ring = smem + S::kOffRing;
+  Bars* bars = reinterpret_cast<Bars*>(smem + S::kOffBar);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int* err = p.err;
+
+  if (PLANNED) pdl_launch();
+  if (threadIdx.x == 0) {
+    ptx::prefetch_tensor_map(&tm_q);
+    ptx::prefetch_tensor_map(&tm_k);
+    ptx::prefetch_tensor_map(&tm_v);
+    for (int i = 0; i < S::kStages; ++i) {
+      ptx::mbar_init(&bars->full[i], 1);
+      ptx::mbar_init(&bars->empty[i], 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      ptx::mbar_init(&bars->q_full[t], 1);
+      ptx::mbar_init(&bars->q_empty[t], 1);
+      ptx::mbar_init(&bars->s_full[t], 1);
+      ptx::mbar_init(&bars->p_ready[t], 4);
+      ptx::mbar_init(&bars->o_full[t], 1);
+      ptx::mbar_init(&bars->o_free[t], 4);
+    }
+    ptx::mbar_init(&bars->drain, 1);
+    ptx::fence_barrier_init();
+  }
+  if (warp == 8) {
+    ptx::tmem_alloc(&bars->tmem, 512);
+    ptx::tmem_relinquish();
+  }
+  if (!PLANNED && warp == 9) {
+    // this CTA's item: the (blockIdx.x / kv_heads)-th of the items in sequence order
+    int want = blockIdx.x / p.kv_heads, found = 0;
+    const int per_item = 2 * p.tile_pos;
+    for (int b0 = 0; b0 < p.batch; b0 += 32) {
+      int q0 = 0, lq = 0, k0 = 0, lk = 0, n = 0;
+      if (b0 + lane < p.batch && sequence(p, b0 + lane, true, q0, lq, k0, lk)) n = (lq + per_item - 1) / per_item;
+      int incl = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += u;
+      }
+      const int i = want - (incl - n);
+      if (i >= 0 && i < n) {
+        const int last = min((i + 1) * per_item, lq) - 1;
+        bars->item = Item{q0, lq, k0, lk, i * per_item, 0, (seen_keys(last, lq, lk, p.causal) + kKeys - 1) / kKeys, -1};
+        found = 1;
+      }
+      want -= __shfl_sync(0xffffffffu, incl, 31);
+    }
+    found = __any_sync(0xffffffffu, found);
+    if (lane == 0) bars->item_ok = found;
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  if (PLANNED) pdl_wait();
+  const uint32_t tmem = bars->tmem;
+  Walk<PLANNED> walk(p, bars);
+  Item it;
+  int hk;
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
+    if (warp == 9 && lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      uint32_t q_uses[2] = {0, 0};
+      long long issued = 0;
+      bool ok = true;
+      while (ok && walk.next(it, hk)) {
+        const int n0 = tile_count(p, it, 0), n1 = tile_count(p, it, 1), n = max(n0, n1);
+        auto load_q = [&](int t) {
+          if (!(ok = ok && ptx::mbar_wait(&bars->q_empty[t], (q_uses[t] & 1) ^ 1, err))) return;
+          ++q_uses[t];
+          ptx::mbar_arrive_expect_tx(&bars->q_full[t], uint32_t(S::kAtoms * p.tile_pos * p.group * 128));
+          for (int a = 0; a < S::kAtoms; ++a)
+            ptx::tma_load_3d(s_q + t * S::kTileBytes + a * 16384, &tm_q, a * 64, hk * p.group,
+                             it.q_row + it.pos + t * p.tile_pos, &bars->q_full[t]);
+        };
+        auto load_kv = [&](const CUtensorMap* map, int j) {
+          if (!(ok = ok && ptx::mbar_wait(&bars->empty[stage], phase ^ 1, err))) return;
+          ptx::mbar_arrive_expect_tx(&bars->full[stage], uint32_t(S::kTileBytes));
+          for (int a = 0; a < S::kAtoms; ++a)
+            ptx::tma_load_2d(s_ring + stage * S::kTileBytes + a * 16384, map, hk * D + a * 64,
+                             it.k_row + (it.t0 + j) * kKeys, &bars->full[stage]);
+          ++issued;
+          if (++stage == S::kStages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        };
+        if (n == 0) continue;
+        if (n0 > 0) load_q(0);
+        load_kv(&tm_k, 0);
+        if (n1 > 0) load_q(1);
+        for (int j = 0; j < n && ok; ++j) {
+          load_kv(&tm_v, j);
+          if (j + 1 < n) load_kv(&tm_k, j + 1);
+        }
+      }
+      // the loads in flight land before the CTA can exit (bounded)
+      auto landed = [&](uint64_t* bar, uint32_t parity) {
+        const unsigned long long t0 = ptx::globaltimer();
+        while (!ptx::mbar_try_wait(bar, parity) && ptx::globaltimer() - t0 < ptx::kTimeoutNs) {
+        }
+      };
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        if (q_uses[t] > 0) landed(&bars->q_full[t], (q_uses[t] - 1) & 1);
+      for (long long j = std::max(0ll, issued - S::kStages); j < issued; ++j)
+        landed(&bars->full[j % S::kStages], uint32_t((j / S::kStages) & 1));
+    }
+    if (warp == 8) {
+    constexpr uint32_t fmt = (E::kMmaFormat << 7) | (E::kMmaFormat << 10);
+    constexpr uint32_t idesc_s = ptx::idesc_f16_f32(128, kKeys) | fmt;
+    constexpr uint32_t idesc_o = ptx::idesc_f16_f32(128, D, 1) | fmt;
+    int stage = 0;
+    uint32_t phase = 0;
+    uint32_t items_of[2] = {0, 0}, p_uses[2] = {0, 0};
+    bool ok = true;
+    while (ok && walk.next(it, hk)) {
+      const int cnt[2] = {tile_count(p, it, 0), tile_count(p, it, 1)};
+      const int n = max(cnt[0], cnt[1]);
+      if (n == 0) continue;
+      auto advance = [&] {
+        if (++stage == S::kStages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      };
+      auto scores = [&](int t, int j, uint32_t k_addr) {
+        const uint32_t q_addr = ptx::smem_u32(s_q + t * S::kTileBytes);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t off = uint32_t(k >> 2) * 16384 + (k & 3) * 32;
+          ptx::umma_f16_ss(tmem + t * 128, ptx::desc_kmajor_sw128(q_addr + off), ptx::desc_kmajor_sw128(k_addr + off), idesc_s,
+                           k != 0);
+        }
+        ptx::umma_commit(&bars->s_full[t]);
+        if (j + 1 == cnt[t]) ptx::umma_commit(&bars->q_empty[t]);
+      };
+      // S_t(0)
+      ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->full[stage], phase, err));
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        if (ok && cnt[t] > 0) {
+          ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->q_full[t], items_of[t] & 1, err));
+          ptx::tc_fence_after();
+          if (ok && lane == 0) scores(t, 0, ptx::smem_u32(s_ring + stage * S::kTileBytes));
+        }
+      if (!ok) break;
+      if (lane == 0) ptx::umma_commit(&bars->empty[stage]);
+      advance();
+      for (int j = 0; j < n && ok; ++j) {
+        const int v_stage = stage;
+        const uint32_t v_phase = phase;
+        advance();
+        ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->full[v_stage], v_phase, err));
+        if (!ok) break;
+        // value rows behind the sequence's last key: zero, whatever the buffer holds there
+        const int valid = it.lk - (it.t0 + j) * kKeys;
+        uint8_t* v_tile = s_ring + v_stage * S::kTileBytes;
+        if (valid < kKeys) {
+          for (int i = lane; i < (kKeys - valid) * 8; i += 32)
+#pragma unroll
+            for (int a = 0; a < S::kAtoms; ++a)
+              *reinterpret_cast<uint4*>(v_tile + a * 16384 + valid * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+          ptx::fence_proxy_async_smem();
+          __syncwarp();
+        }
+        const bool more = j + 1 < n;
+        bool k_ready = false;
+        const uint32_t v_addr = ptx::smem_u32(v_tile);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (!ok || j >= cnt[t]) continue;
+          ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->p_ready[t], p_uses[t] & 1, err));
+          ++p_uses[t];
+          if (ok && j == 0) ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->o_free[t], (items_of[t] & 1) ^ 1, err));
+          if (!ok) continue;
+          ptx::tc_fence_after();
+          if (lane == 0) {
+#pragma unroll
+            for (int k = 0; k < kKeys / 16; ++k)
+              ptx::umma_f16_ts(tmem + 256 + t * D, tmem + t * 128 + k * 8, desc_v(v_addr + k * 2048), idesc_o, (j | k) != 0);
+          }
+          if (j + 1 < cnt[t]) {
+            if (!k_ready) {
+              ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->full[stage], phase, err));
+              if (!ok) continue;
+              ptx::tc_fence_after();
+              k_ready = true;
+            }
+            if (lane == 0) scores(t, j + 1, ptx::smem_u32(s_ring + stage * S::kTileBytes));
+          } else {
+            if (lane == 0) ptx::umma_commit(&bars->o_full[t]);
+          }
+        }
+        if (!ok) break;
+        if (lane == 0) ptx::umma_commit(&bars->empty[v_stage]);
+        if (more) {
+          if (lane == 0) ptx::umma_commit(&bars->empty[stage]);
+          advance();
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        if (cnt[t] > 0) ++items_of[t];
+    }
+    if (lane == 0) {
+      // every issued MMA is done before TMEM is released
+      ptx::umma_commit(&bars->drain);
+      const unsigned long long t0 = ptx::globaltimer();
+      while (!ptx::mbar_try_wait(&bars->drain, 0) && ptx::globaltimer() - t0 < ptx::kTimeoutNs) {
+      }
+    }
+    }
+    __syncwarp();
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRowRegs));
+    const int t = warp >> 2;
+    const int r = (warp & 3) * 32 + lane;
+    const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + t * 128 + lanes, t_o = tmem + 256 + t * D + lanes;
+    const int row_pos = r / p.group, row_head = r % p.group;
+    const int warp_pos = ((warp & 3) * 32) / p.group;
+    const float c = p.scale_log2;
+    uint32_t s_uses = 0, items_done = 0;
+    bool ok = true;
+    while (ok && walk.next(it, hk)) {
+      const int n = tile_count(p, it, t);
+      const int pos = it.pos + t * p.tile_pos + row_pos;
+      const bool live = row_pos < p.tile_pos && pos < it.lq;
+      const int seen = live ? seen_keys(pos, it.lq, it.lk, p.causal) : 0;
+      const int warp_seen = seen_keys(min(it.pos + t * p.tile_pos + warp_pos, it.lq - 1), it.lq, it.lk, p.causal);
+      float m = -INFINITY, mc = 0.f;
+      float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
+      for (int j = 0; j < n; ++j) {
+        ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->s_full[t], s_uses & 1, err));
+        ++s_uses;
+        if (!ok) break;
+        ptx::tc_fence_after();
+        uint32_t s[4][32];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ptx::tmem_ld_32x32b_x32(t_s + i * 32, s[i]);
+        ptx::tmem_wait_ld();
+        const int key0 = (it.t0 + j) * kKeys;
+        if (key0 + kKeys > warp_seen) {  // some row of the warp does not see the whole tile
+          const int vis = seen - key0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (i * 32 + e >= vis) s[i][e] = 0xff800000u;
+        }
+        float mx[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          mx[i] = __uint_as_float(s[i][0]);
+#pragma unroll
+          for (int e = 1; e < 31; e += 2) mx[i] = max3_nan(mx[i], __uint_as_float(s[i][e]), __uint_as_float(s[i][e + 1]));
+          mx[i] = max3_nan(mx[i], __uint_as_float(s[i][31]), __uint_as_float(s[i][31]));
+        }
+        const float top = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], m);
+        if (j == 0) {
+          m = top;
+          mc = m == -INFINITY ? 0.f : m * c;
+        } else {
+          const bool grow = !((top - m) * c <= kGrowth) && top != m;
+          if (__any_sync(0xffffffffu, grow)) {
+            const float f = grow ? ex2(m * c - top * c) : 1.f;
+            if (grow) {
+              m = top;
+              mc = m * c;
+            }
+            sum0.x *= f;
+            sum0.y *= f;
+            sum1.x *= f;
+            sum1.y *= f;
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) {
+              uint32_t o[32];
+              ptx::tmem_ld_32x32b_x32(t_o + i * 32, o);
+              ptx::tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              ptx::tmem_st_32x32b_x32(t_o + i * 32, o);
+            }
+          }
+        }
+        const float2 c2 = make_float2(c, c), mc2 = make_float2(-mc, -mc);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t w[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float2 x = __ffma2_rn(make_float2(__uint_as_float(s[i][2 * e]), __uint_as_float(s[i][2 * e + 1])), c2, mc2);
+            x.x = ex2(x.x);
+            x.y = ex2(x.y);
+            if (e & 1)
+              sum1 = __fadd2_rn(sum1, x);
+            else
+              sum0 = __fadd2_rn(sum0, x);
+            w[e] = E::pack(x.x, x.y);
+          }
+          ptx::tmem_st_32x32b_x16(t_s + i * 16, w);
+        }
+        ptx::tmem_wait_st();
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&bars->p_ready[t]);
+      }
+      if (!ok) break;
+      // ---- the item's rows of this tile
+      const float l = (sum0.x + sum0.y) + (sum1.x + sum1.y);
+      if (n > 0) {
+        ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->o_full[t], items_done & 1, err));
+        if (!ok) break;
+        ptx::tc_fence_after();
+      }
+      const int head = hk * p.group + row_head;
+      if (it.slot < 0) {
+        const float inv = seen > 0 ? 1.f / l : 0.f;
+        T* dst = static_cast<T*>(p.out) + (long long)(it.q_row + pos) * p.ldo + head * D;
+        float bad = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          uint32_t o[32];
+          if (n > 0) {
+            ptx::tmem_ld_32x32b_x32(t_o + i * 32, o);
+            ptx::tmem_wait_ld();
+          }
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const float x = seen > 0 ? __uint_as_float(o[e]) * inv : 0.f;
+            bad = fmaf(x, 0.f, bad);  // NaN as soon as one value is not finite
+            o[e] = __float_as_uint(x);
+          }
+          if (live) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t* w = o + e * 8;
+              *reinterpret_cast<uint4*>(dst + i * 32 + e * 8) =
+                  make_uint4(E::pack(__uint_as_float(w[0]), __uint_as_float(w[1])), E::pack(__uint_as_float(w[2]), __uint_as_float(w[3])),
+                             E::pack(__uint_as_float(w[4]), __uint_as_float(w[5])), E::pack(__uint_as_float(w[6]), __uint_as_float(w[7])));
+            }
+          }
+        }
+        uint32_t again = __ballot_sync(0xffffffffu, live && bad != 0.f);
+        while (again != 0) {  // rare: a result that is not finite
+          const int src = __ffs(again) - 1;
+          again &= again - 1;
+          store_row_by_definition<T, D>(p, it.q_row, it.lq, it.k_row, it.lk, __shfl_sync(0xffffffffu, pos, src),
+                                        __shfl_sync(0xffffffffu, head, src));
+        }
+      } else {
+        const long long at = ((long long)it.slot * p.kv_heads + hk) * p.rows_cap + t * p.tile_pos * p.group + r;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          uint32_t o[32];
+          if (n > 0) {
+            ptx::tmem_ld_32x32b_x32(t_o + i * 32, o);
+            ptx::tmem_wait_ld();
+          }
+          if (live) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              *reinterpret_cast<uint4*>(p.part_o + at * D + i * 32 + e * 4) =
+                  n > 0 ? make_uint4(o[e * 4], o[e * 4 + 1], o[e * 4 + 2], o[e * 4 + 3]) : make_uint4(0, 0, 0, 0);
+          }
+        }
+        if (live) p.part_ml[at] = make_float2(m, l);
+      }
+      if (n > 0) {
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&bars->o_free[t]);
+        ++items_done;
+      }
+    }
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the partial rows of split items: weights 2^(c m_s - c m) of the splits, one warp a row.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) combine_kernel(const Params p) {
+  using E = ElemOps<T>;
+  constexpr int PER = D / 32;
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int rows_per_item = 2 * p.tile_pos * p.group;
+  const long long total = (long long)p.header->n_splits * p.kv_heads * p.rows_cap;
+  for (long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); w < total; w += (long long)gridDim.x * 8) {
+    const int row = int(w % p.rows_cap);
+    const int hk = int(w / p.rows_cap % p.kv_heads);
+    const SplitItem it = p.splits[w / p.rows_cap / p.kv_heads];
+    if (row >= rows_per_item) continue;
+    const int pos = it.pos + row / p.group, head = hk * p.group + row % p.group;
+    if (pos >= it.lq) continue;
+    float m = -INFINITY;
+    for (int s = lane; s < it.n; s += 32) {
+      const float ms = p.part_ml[((long long)(it.slot + s) * p.kv_heads + hk) * p.rows_cap + row].x;
+      m = max3_nan(m, ms, ms);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const float u = __shfl_xor_sync(0xffffffffu, m, o);
+      m = max3_nan(m, u, u);
+    }
+    const float mc = m == -INFINITY ? 0.f : m * p.scale_log2;
+    float acc[PER] = {}, l = 0.f;
+    for (int s = 0; s < it.n; ++s) {
+      const long long at = ((long long)(it.slot + s) * p.kv_heads + hk) * p.rows_cap + row;
+      const float2 ml = p.part_ml[at];
+      const float f = ml.x == -INFINITY ? 0.f : ex2(fmaf(ml.x, p.scale_log2, -mc));
+      l = fmaf(f, ml.y, l);
+      const float* src = p.part_o + at * D + lane * PER;
+#pragma unroll
+      for (int i = 0; i < PER; i += 2) {
+        const float2 v = *reinterpret_cast<const float2*>(src + i);
+        acc[i] = fmaf(f, v.x, acc[i]);
+        acc[i + 1] = fmaf(f, v.y, acc[i + 1]);
+      }
+    }
+    const int seen = seen_keys(pos, it.lq, it.lk, p.causal);
+    const float inv = seen > 0 ? 1.f / l : 0.f;
+    float bad = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      acc[i] = seen > 0 ? acc[i] * inv : 0.f;
+      bad = fmaf(acc[i], 0.f, bad);
+    }
+    if (__any_sync(0xffffffffu, bad != 0.f)) row_by_definition<T, D>(p, it.q_row, it.lq, it.k_row, it.lk, pos, head, acc);
+    uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + (long long)(it.q_row + pos) * p.ldo + head * D + lane * PER);
+#pragma unroll
+    for (int i = 0; i < PER / 2; ++i) dst[i] = E::pack(acc[2 * i], acc[2 * i + 1]);
+  }
+}
+
+// ------------------------------------------------------------------------------------- host
+
+// 16-bit tensor map with 128-byte swizzled boxes of 64 columns.
+gdc_status encode(CUtensorMap* map, bool bf16, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+                  const cuuint32_t* box) {
+  auto fn = get_encode_fn();
+  if (!fn) return set_error(GDC_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r =
+      fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, cuuint32_t(rank), const_cast<void*>(base), dims,
+         strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(GDC_ERR_CUDA, "cuTensorMapEncodeTiled (packed attention) failed (%d)", int(r));
+  return GDC_OK;
+}
+
+// Launch whose kernel may start while the kernel before it on the stream still runs; it waits for
+// that one's results itself (griddepcontrol.wait).
+template <typename... KArgs, typename... Args>
+cudaError_t launch_after(void (*kern)(KArgs...), int grid, int threads, size_t smem, cudaStream_t stream, Args... args) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(grid));
+  cfg.blockDim = dim3(unsigned(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
+template <typename T, int D>
+gdc_status launch_typed(const PackedAttentionArgs& a, cudaStream_t stream, int* err) {
+  using S = Shape<D>;
+  constexpr bool bf16 = ElemOps<T>::kMmaFormat == 1;
+  int dev = 0;
+  GDC_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64) return set_error(GDC_ERR_CUDA, "device ordinal out of range");
+  const PlanLayout l = plan_layout(a.batch, a.q_rows, a.k_rows, a.heads, a.kv_heads, D);
+  const int sms = device_sm_count(dev);
+  const int group = a.heads / a.kv_heads, tile_pos = kKeys / group;
+
+  CUtensorMap tq, tk, tv;
+  {
+    const cuuint64_t dims[3] = {D, cuuint64_t(a.heads), cuuint64_t(a.q_rows)};
+    const cuuint64_t strides[2] = {D * 2, cuuint64_t(a.ldq) * 2};
+    const cuuint32_t box[3] = {64, cuuint32_t(group), cuuint32_t(tile_pos)};
+    GDC_TRY(encode(&tq, bf16, a.q, 3, dims, strides, box));
+  }
+  // without keys nothing is loaded; the maps then describe the queries
+  const bool keys = a.k_rows > 0;
+  for (int i = 0; i < 2; ++i) {
+    const cuuint64_t dims[2] = {cuuint64_t(keys ? a.kv_heads : a.heads) * D, cuuint64_t(keys ? a.k_rows : a.q_rows)};
+    const cuuint64_t strides[1] = {cuuint64_t(keys ? (i ? a.ldv : a.ldk) : a.ldq) * 2};
+    const cuuint32_t box[2] = {64, kKeys};
+    GDC_TRY(encode(i ? &tv : &tk, bf16, keys ? (i ? a.v : a.k) : a.q, 2, dims, strides, box));
+  }
+  Params p{};
+  p.q = a.q;
+  p.k = a.k;
+  p.v = a.v;
+  p.out = a.out;
+  p.ldq = a.ldq;
+  p.ldk = a.ldk;
+  p.ldv = a.ldv;
+  p.ldo = a.ldo;
+  p.q_off = a.q_off;
+  p.k_off = a.k_off;
+  p.batch = a.batch;
+  p.q_rows = int(a.q_rows);
+  p.k_rows = int(a.k_rows);
+  p.heads = a.heads;
+  p.kv_heads = a.kv_heads;
+  p.group = group;
+  p.tile_pos = tile_pos;
+  p.causal = a.causal;
+  p.scale = a.scale;
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  p.header = reinterpret_cast<PlanHeader*>(a.workspace);
+  p.items = reinterpret_cast<Item*>(a.workspace + l.items_at);
+  p.splits = reinterpret_cast<SplitItem*>(a.workspace + l.splits_at);
+  p.part_o = reinterpret_cast<float*>(a.workspace + l.part_o_at);
+  p.part_ml = reinterpret_cast<float2*>(a.workspace + l.part_ml_at);
+  p.rows_cap = l.rows_cap;
+  p.chunks_cap = l.chunks_cap;
+  p.splits_cap = l.split ? int(l.items_ub) : 0;
+  p.can_split = l.split;
+  p.err = err;
+
+  static PerDeviceOnce configured;
+  const cudaError_t ce = cudaError_t(per_device_once(configured, dev, [&] {
+    const cudaError_t e = cudaFuncSetAttribute(packed_attention_kernel<T, D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmemBytes);
+    return e != cudaSuccess ? e
+                            : cudaFuncSetAttribute(packed_attention_kernel<T, D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   S::kSmemBytes);
+  }));
+  if (ce != cudaSuccess) return set_error(GDC_ERR_CUDA, "packed attention smem attribute: %s", cudaGetErrorString(ce));
+  if (!l.planned) {
+    packed_attention_kernel<T, D, false><<<unsigned(l.items_ub * a.kv_heads), kThreads, S::kSmemBytes, stream>>>(tq, tk, tv, p);
+    return check_launch("packed_attention_kernel");
+  }
+  plan_kernel<<<1, kPlanThreads, 0, stream>>>(p);
+  GDC_TRY(check_launch("plan_kernel"));
+  const int64_t jobs = int64_t(l.chunks_cap) * a.kv_heads;
+  GDC_CUDA_TRY(launch_after(packed_attention_kernel<T, D, true>, int(std::min<int64_t>(sms, jobs)), kThreads, S::kSmemBytes, stream, tq,
+                            tk, tv, p));
+  if (l.split) {
+    const int64_t rows = l.items_ub * a.kv_heads * l.rows_cap;
+    GDC_CUDA_TRY(launch_after(combine_kernel<T, D>, int(std::min<int64_t>(4 * sms, (rows + 7) / 8)), 256, 0, stream, p));
+  }
+  return GDC_OK;
 }
 
 }  // namespace
 
-size_t packed_attention_workspace(int, int64_t, int64_t, int, int, int) { return 256; }
+size_t packed_attention_workspace(int batch, int64_t q_rows, int64_t k_rows, int heads, int kv_heads, int dim) {
+  if (batch <= 0 || q_rows <= 0) return 0;
+  return plan_layout(batch, q_rows, k_rows, heads, kv_heads, dim).bytes;
+}
 
 gdc_status launch_packed_attention(Elem t, const PackedAttentionArgs& a, cudaStream_t stream, int* err) {
-  const int64_t items = a.q_rows * a.heads > a.batch ? a.q_rows * a.heads : a.batch;
-  const unsigned blocks = unsigned((items + 3) / 4);
-  if (t == Elem::kF16) {
-    if (a.dim == 64) packed_attention_rows_kernel<__half, 64><<<blocks, 128, 0, stream>>>(a, err);
-    else packed_attention_rows_kernel<__half, 128><<<blocks, 128, 0, stream>>>(a, err);
-  } else {
-    if (a.dim == 64) packed_attention_rows_kernel<__nv_bfloat16, 64><<<blocks, 128, 0, stream>>>(a, err);
-    else packed_attention_rows_kernel<__nv_bfloat16, 128><<<blocks, 128, 0, stream>>>(a, err);
-  }
-  return check_launch("packed_attention_rows_kernel");
+  if (t == Elem::kF16)
+    return a.dim == 64 ? launch_typed<__half, 64>(a, stream, err) : launch_typed<__half, 128>(a, stream, err);
+  return a.dim == 64 ? launch_typed<__nv_bfloat16, 64>(a, stream, err) : launch_typed<__nv_bfloat16, 128>(a, stream, err);
 }
 
 }  // namespace gdc
