@@ -65,6 +65,10 @@ struct Item {
   int t0, t1;      // key tiles [t0, t1)
   int slot;        // partial rows' slot, -1: the item's only range
 };
+struct Job {  // an item and the key head to do it for
+  Item it;
+  int hk, more, pad[2];  // more: 0 ends the CTA's work
+};
 struct SplitItem {  // an item whose key range was split: slots [slot, slot + n)
   int q_row, lq, k_row, lk, pos, slot, n, pad;
 };
@@ -333,9 +337,9 @@ struct Shape {
 struct Bars {
   uint64_t full[10], empty[10];
   uint64_t q_full[2], q_empty[2], s_full[2], p_ready[2], o_full[2], o_free[2], drain;
-  uint32_t tmem;
-  int item_ok;
-  Item item;
+  uint64_t job_full[2], job_empty[2];
+  uint32_t tmem, pad;
+  Job job[2];
 };
 static_assert(sizeof(Bars) <= 512, "barrier block");
 
@@ -359,33 +363,68 @@ __device__ __forceinline__ int tile_count(const Params& p, const Item& it, int t
   return max(0, min(it.t1, need) - it.t0);
 }
 
-// Walks a CTA's items: planned ones from the list, every other round backwards (the list is in
-// descending cost, so a CTA's share evens out); the unplanned one from shared memory.
-template <bool PLANNED>
-struct Walk {
-  const Params& p;
-  const Bars* bars;
-  long long jobs;
-  int round = 0;
-  __device__ Walk(const Params& p_, const Bars* b) : p(p_), bars(b) {
-    jobs = PLANNED ? (long long)p.header->n_items * p.kv_heads : 1;
-  }
-  __device__ __forceinline__ bool next(Item& it, int& hk) {
-    if (PLANNED) {
-      const long long g = gridDim.x;
-      const long long at = (long long)round * g + ((round & 1) ? g - 1 - blockIdx.x : blockIdx.x);
-      ++round;
-      if (at >= jobs) return false;  // only in the last round: earlier ones are full
-      const int4* src = reinterpret_cast<const int4*>(p.items + at / p.kv_heads);
-      const int4 a = src[0], b = src[1];
-      it = Item{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-      hk = int(at % p.kv_heads);
+// The CTA's next job, by its producer (one lane): planned ones from the list, every other round
+// backwards (the list is in descending cost, so a CTA's share evens out).
+__device__ __forceinline__ bool next_planned(const Params& p, int round, Job& job) {
+  const long long g = gridDim.x;
+  const long long at = (long long)round * g + ((round & 1) ? g - 1 - blockIdx.x : blockIdx.x);
+  if (at >= (long long)p.header->n_items * p.kv_heads) return false;  // only in the last round: earlier ones are full
+  const int4* src = reinterpret_cast<const int4*>(p.items + at / p.kv_heads);
+  const int4 a = src[0], b = src[1];
+  job.it = Item{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  job.hk = int(at % p.kv_heads);
+  return true;
+}
+
+// The unplanned job of this CTA: the (blockIdx.x / kv_heads)-th item in sequence order. One warp;
+// the result is the same in every lane.
+__device__ __forceinline__ bool find_job(const Params& p, Job& job) {
+  const int lane = threadIdx.x & 31, per_item = 2 * p.tile_pos;
+  int want = blockIdx.x / p.kv_heads;
+  job.hk = blockIdx.x % p.kv_heads;
+  for (int b0 = 0; b0 < p.batch; b0 += 32) {
+    int q0 = 0, lq = 0, k0 = 0, lk = 0, n = 0;
+    if (b0 + lane < p.batch && sequence(p, b0 + lane, true, q0, lq, k0, lk)) n = (lq + per_item - 1) / per_item;
+    int incl = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += u;
+    }
+    const int i = want - (incl - n);
+    const uint32_t hit = __ballot_sync(0xffffffffu, i >= 0 && i < n);
+    if (hit != 0) {
+      const int src = __ffs(hit) - 1;
+      Item& it = job.it;
+      it.q_row = __shfl_sync(0xffffffffu, q0, src);
+      it.lq = __shfl_sync(0xffffffffu, lq, src);
+      it.k_row = __shfl_sync(0xffffffffu, k0, src);
+      it.lk = __shfl_sync(0xffffffffu, lk, src);
+      it.pos = __shfl_sync(0xffffffffu, i, src) * per_item;
+      it.t0 = 0;
+      it.t1 = (seen_keys(min(it.pos + per_item, it.lq) - 1, it.lq, it.lk, p.causal) + kKeys - 1) / kKeys;
+      it.slot = -1;
       return true;
     }
-    if (round++ > 0 || !bars->item_ok) return false;
-    it = bars->item;
-    hk = blockIdx.x % p.kv_heads;
-    return true;
+    want -= __shfl_sync(0xffffffffu, incl, 31);
+  }
+  return false;
+}
+
+// A consumer's view of the job ring.
+struct Jobs {
+  Bars* bars;
+  uint32_t n = 0;
+  // Waits for the next job (all lanes of a warp); null: no more, or a wait gave up.
+  __device__ __forceinline__ const Job* next(int* err) {
+    if (!__all_sync(0xffffffffu, ptx::mbar_wait(&bars->job_full[n & 1], (n >> 1) & 1, err))) return nullptr;
+    const Job* job = &bars->job[n & 1];
+    return job->more ? job : nullptr;
+  }
+  __device__ __forceinline__ void done() {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(&bars->job_empty[n & 1]);
+    ++n;
   }
 };
 
@@ -420,6 +459,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       ptx::mbar_init(&bars->o_full[t], 1);
       ptx::mbar_init(&bars->o_free[t], 4);
     }
+    for (int i = 0; i < 2; ++i) {
+      ptx::mbar_init(&bars->job_full[i], 1);
+      ptx::mbar_init(&bars->job_empty[i], 9);  // the MMA warp and the eight row warps
+    }
     ptx::mbar_init(&bars->drain, 1);
     ptx::fence_barrier_init();
   }
@@ -427,48 +470,36 @@ __global__ void __launch_bounds__(kThreads, 1)
     ptx::tmem_alloc(&bars->tmem, 512);
     ptx::tmem_relinquish();
   }
-  if (!PLANNED && warp == 9) {
-    // this CTA's item: the (blockIdx.x / kv_heads)-th of the items in sequence order
-    int want = blockIdx.x / p.kv_heads, found = 0;
-    const int per_item = 2 * p.tile_pos;
-    for (int b0 = 0; b0 < p.batch; b0 += 32) {
-      int q0 = 0, lq = 0, k0 = 0, lk = 0, n = 0;
-      if (b0 + lane < p.batch && sequence(p, b0 + lane, true, q0, lq, k0, lk)) n = (lq + per_item - 1) / per_item;
-      int incl = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += u;
-      }
-      const int i = want - (incl - n);
-      if (i >= 0 && i < n) {
-        const int last = min((i + 1) * per_item, lq) - 1;
-        bars->item = Item{q0, lq, k0, lk, i * per_item, 0, (seen_keys(last, lq, lk, p.causal) + kKeys - 1) / kKeys, -1};
-        found = 1;
-      }
-      want -= __shfl_sync(0xffffffffu, incl, 31);
-    }
-    found = __any_sync(0xffffffffu, found);
-    if (lane == 0) bars->item_ok = found;
-  }
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
   if (PLANNED) pdl_wait();
   const uint32_t tmem = bars->tmem;
-  Walk<PLANNED> walk(p, bars);
-  Item it;
-  int hk;
+  Jobs jobs{bars};
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
-    if (warp == 9 && lane == 0) {
+    if (warp == 9) {
+      Job job;
+      const bool found = PLANNED || find_job(p, job);
+      if (lane == 0) {
       int stage = 0;
       uint32_t phase = 0;
       uint32_t q_uses[2] = {0, 0};
       long long issued = 0;
       bool ok = true;
-      while (ok && walk.next(it, hk)) {
+      for (int round = 0; ok; ++round) {
+        if (PLANNED)
+          job.more = next_planned(p, round, job);
+        else
+          job.more = found && round == 0;
+        Bars* b = bars;
+        if (!(ok = ptx::mbar_wait(&b->job_empty[round & 1], ((round >> 1) & 1) ^ 1, err))) break;
+        b->job[round & 1] = job;
+        ptx::mbar_arrive(&b->job_full[round & 1]);
+        if (!job.more) break;
+        const Item& it = job.it;
+        const int hk = job.hk;
         const int n0 = tile_count(p, it, 0), n1 = tile_count(p, it, 1), n = max(n0, n1);
         auto load_q = [&](int t) {
           if (!(ok = ok && ptx::mbar_wait(&bars->q_empty[t], (q_uses[t] & 1) ^ 1, err))) return;
@@ -510,6 +541,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (q_uses[t] > 0) landed(&bars->q_full[t], (q_uses[t] - 1) & 1);
       for (long long j = std::max(0ll, issued - S::kStages); j < issued; ++j)
         landed(&bars->full[j % S::kStages], uint32_t((j / S::kStages) & 1));
+      }
     }
     if (warp == 8) {
     constexpr uint32_t fmt = (E::kMmaFormat << 7) | (E::kMmaFormat << 10);
@@ -519,9 +551,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t phase = 0;
     uint32_t items_of[2] = {0, 0}, p_uses[2] = {0, 0};
     bool ok = true;
-    while (ok && walk.next(it, hk)) {
-      const int cnt[2] = {tile_count(p, it, 0), tile_count(p, it, 1)};
+    while (ok) {
+      const Job* job = jobs.next(err);
+      if (job == nullptr) break;
+      const int cnt[2] = {tile_count(p, job->it, 0), tile_count(p, job->it, 1)};
       const int n = max(cnt[0], cnt[1]);
+      const int keys_left = job->it.lk - job->it.t0 * kKeys;
+      jobs.done();
       if (n == 0) continue;
       auto advance = [&] {
         if (++stage == S::kStages) {
@@ -559,7 +595,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->full[v_stage], v_phase, err));
         if (!ok) break;
         // value rows behind the sequence's last key: zero, whatever the buffer holds there
-        const int valid = it.lk - (it.t0 + j) * kKeys;
+        const int valid = keys_left - j * kKeys;
         uint8_t* v_tile = s_ring + v_stage * S::kTileBytes;
         if (valid < kKeys) {
           for (int i = lane; i < (kKeys - valid) * 8; i += 32)
@@ -628,12 +664,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float c = p.scale_log2;
     uint32_t s_uses = 0, items_done = 0;
     bool ok = true;
-    while (ok && walk.next(it, hk)) {
-      const int n = tile_count(p, it, t);
-      const int pos = it.pos + t * p.tile_pos + row_pos;
-      const bool live = row_pos < p.tile_pos && pos < it.lq;
-      const int seen = live ? seen_keys(pos, it.lq, it.lk, p.causal) : 0;
-      const int warp_seen = seen_keys(min(it.pos + t * p.tile_pos + warp_pos, it.lq - 1), it.lq, it.lk, p.causal);
+    while (true) {
+      const Job* job = jobs.next(err);
+      if (job == nullptr) break;
+      int n, rel, warp_rel;  // key tiles; keys that the row, and the warp's first row, see from the range's first on
+      {
+        const Item& it = job->it;
+        n = tile_count(p, it, t);
+        const int pos = it.pos + t * p.tile_pos + row_pos;
+        rel = (row_pos < p.tile_pos && pos < it.lq ? seen_keys(pos, it.lq, it.lk, p.causal) : 0) - it.t0 * kKeys;
+        warp_rel = seen_keys(min(it.pos + t * p.tile_pos + warp_pos, it.lq - 1), it.lq, it.lk, p.causal) - it.t0 * kKeys;
+      }
       float m = -INFINITY, mc = 0.f;
       float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
       for (int j = 0; j < n; ++j) {
@@ -645,9 +686,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < 4; ++i) ptx::tmem_ld_32x32b_x32(t_s + i * 32, s[i]);
         ptx::tmem_wait_ld();
-        const int key0 = (it.t0 + j) * kKeys;
-        if (key0 + kKeys > warp_seen) {  // some row of the warp does not see the whole tile
-          const int vis = seen - key0;
+        if ((j + 1) * kKeys > warp_rel) {  // some row of the warp does not see the whole tile
+          const int vis = rel - j * kKeys;
 #pragma unroll
           for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -678,14 +718,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             sum0.y *= f;
             sum1.x *= f;
             sum1.y *= f;
-#pragma unroll
-            for (int i = 0; i < D / 32; ++i) {
-              uint32_t o[32];
-              ptx::tmem_ld_32x32b_x32(t_o + i * 32, o);
+#pragma unroll 1
+            for (int i = 0; i < D / 16; ++i) {  // rare: few registers beside the scores
+              uint32_t o[16];
+              ptx::tmem_ld_32x32b_x16(t_o + i * 16, o);
               ptx::tmem_wait_ld();
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-              ptx::tmem_st_32x32b_x32(t_o + i * 32, o);
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              ptx::tmem_st_32x32b_x16(t_o + i * 16, o);
             }
           }
         }
@@ -719,7 +759,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         ptx::tc_fence_after();
       }
-      const int head = hk * p.group + row_head;
+      const Item it = job->it;
+      const int hk = job->hk;
+      const int head = hk * p.group + row_head, pos = it.pos + t * p.tile_pos + row_pos;
+      const bool live = row_pos < p.tile_pos && pos < it.lq;
+      const int seen = live ? seen_keys(pos, it.lq, it.lk, p.causal) : 0;
       if (it.slot < 0) {
         const float inv = seen > 0 ? 1.f / l : 0.f;
         T* dst = static_cast<T*>(p.out) + (long long)(it.q_row + pos) * p.ldo + head * D;
@@ -778,6 +822,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) ptx::mbar_arrive(&bars->o_free[t]);
         ++items_done;
       }
+      jobs.done();
     }
   }
   ptx::tc_fence_before();
