@@ -1,70 +1,491 @@
-// out = residual + act(a . w^T + bias): tiled on CUDA cores, fp32 sums.
+// out = residual + act(a . w^T + bias) on tcgen05 tensor cores, any M, N and K.
+//
+// The product is computed transposed: the MMA's 128 rows are weight rows (output columns n) and
+// its N dimension is `bt` rows of a (m), bt a multiple of 16 up to 256 chosen per call. So
+//   * few rows of a cost a narrow MMA (bt = 16 for a single token) while the weights, which are
+//     then all the traffic, stream through the wide operand;
+//   * in the epilogue a thread owns one n (its bias is one register) and walks over m: a warp
+//     reads residuals and writes results 32 neighbouring n at a time, 64 bytes a row, at any
+//     alignment, pitch and width, and a row count only the device knows limits a loop.
+//
+// Two forms, one kernel:
+//   PAIR    two CTAs (cta_group::2) make a 256 (n) x bt (m) tile: each loads its 128 weight rows
+//           and half of the a rows, the leader issues the MMAs for both. Persistent, two
+//           accumulators in TMEM, so a tile's epilogue runs beside the next tile's products.
+//   single  a CTA makes a 128 x bt tile; where tiles are fewer than SMs, a cluster of 2, 4 or 8 CTAs
+//           splits K, and each sums its share of the columns from all of them, in rank order,
+//           through distributed shared memory.
+//
+// Roles: warp 0 TMA (128-column K blocks of w and a into a ring), warp 1 MMA issue, warps 2-9
+// epilogue (TMEM lane quarter warp % 4; two warps a quarter take alternate 16-column chunks).
+// Sums are fp32 over K in order (K split: in order inside a share, shares in rank order): the
+// same call gives the same bits.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+
 #include "elem.cuh"
+#include "gelu.cuh"
 #include "kernels.h"
+#include "ptx.cuh"
 
 namespace gdc {
+
+PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn();
+
 namespace {
 
-constexpr int kTile = 64, kStep = 16;
+constexpr int kBK = 128;         // K columns of a stage: two 128-byte swizzle atoms an operand
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = 64 + 32 * kEpiWarps;
+constexpr int kMaxStages = 6;
+constexpr int kWBytes = 128 * kBK * 2;
+constexpr int kRingBytes = 192 * 1024;
+constexpr int kMaxSplitBt = 64;  // split K: columns x 128 lanes x 4 bytes of partial sums, 32 KB
+constexpr int kRedBytes = kMaxSplitBt * 512;
+constexpr int kSmemBytes = kRingBytes + kRedBytes + 1024 + 256;
 
-__device__ __forceinline__ float activate(float z, int act) {
-  if (act == kActGelu) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-  if (act == kActRelu) return z > 0.f ? z : (z != z ? z : 0.f);
-  if (act == kActSilu) return z / (1.f + expf(-z));
+struct LinearParams {
+  const void *bias, *residual;
+  void* out;
+  long long ldr, ldo, m_cap;
+  const int32_t* rows_dev;
+  int N, K, act, bt, split, stages, stage_bytes;
+  int* err;
+};
+
+// Tile t of num_n x num_m: groups of 8 n tiles, so that the tiles in flight share both operands.
+__device__ __forceinline__ void tile_at(long long t, int num_n, int num_m, int& nb, int& mb) {
+  const long long per_group = 8ll * num_m;
+  const int g = int(t / per_group);
+  const int width = min(8, num_n - g * 8);
+  const int u = int(t - g * per_group);
+  nb = g * 8 + u % width;
+  mb = u / width;
+}
+
+// The activation of two values (rows m, m + 1 of one n).
+__device__ __forceinline__ float2 activate(float2 z, int act) {
+  if (act == kActGelu) {
+    const float2 g = gelu_erf2(z);
+    return make_float2(z.x > 16.f ? z.x : g.x, z.y > 16.f ? z.y : g.y);  // GELU(x) = x there; keeps +inf
+  }
+  if (act == kActRelu) {
+    asm("max.NaN.f32 %0, %0, 0f00000000;" : "+f"(z.x));
+    asm("max.NaN.f32 %0, %0, 0f00000000;" : "+f"(z.y));
+    return z;
+  }
+  if (act == kActSilu)
+    return make_float2(__fdividef(z.x, 1.f + ex2_approx_f32(-kGeluLog2e * z.x)),
+                       __fdividef(z.y, 1.f + ex2_approx_f32(-kGeluLog2e * z.y)));
   return z;
 }
 
+// One chunk of 16 rows m0.. of column n: residuals are fetched ahead (fetch), then joined with the
+// accumulators and stored.
 template <typename T>
-__global__ void __launch_bounds__(256)
-    linear_residual_kernel(const T* __restrict__ a, const T* __restrict__ w, const T* __restrict__ bias, const T* residual,
-                           T* out, long long lda, long long ldw, long long ldr, long long ldo, long long m_cap,
-                           const int32_t* __restrict__ rows_dev, int N, int K, int act) {
+struct Column {
   using E = ElemOps<T>;
-  __shared__ float sa[kStep][kTile + 1], sw[kStep][kTile + 1];
-  const long long M = rows_dev != nullptr ? min(m_cap, (long long)*rows_dev) : m_cap;
-  const long long m0 = (long long)blockIdx.x * kTile;
-  const int n0 = blockIdx.y * kTile;
-  if (m0 >= M) return;
-  const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
-  float acc[4][4] = {};
-  for (int k0 = 0; k0 < K; k0 += kStep) {
-    for (int i = threadIdx.x; i < kTile * kStep; i += 256) {
-      const int r = i / kStep, k = i % kStep;
-      sa[k][r] = m0 + r < M && k0 + k < K ? E::to_f32(a[(m0 + r) * lda + k0 + k]) : 0.f;
-      sw[k][r] = n0 + r < N && k0 + k < K ? E::to_f32(w[(long long)(n0 + r) * ldw + k0 + k]) : 0.f;
-    }
-    __syncthreads();
-    for (int k = 0; k < kStep; ++k)
-      for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sa[k][ty + 16 * i], sw[k][tx + 16 * j], acc[i][j]);
-    __syncthreads();
+  const T* res;
+  T* out;
+  long long ldr, ldo, M;
+  float bias;
+  int act;
+  bool live;
+  __device__ __forceinline__ void fetch(long long m0, uint16_t (&r)[16]) const {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      r[i] = res != nullptr && live && m0 + i < M ? *reinterpret_cast<const uint16_t*>(res + (m0 + i) * ldr) : uint16_t(0);
   }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const long long m = m0 + ty + 16 * i;
-      const int n = n0 + tx + 16 * j;
-      if (m >= M || n >= N) continue;
-      float z = activate(acc[i][j] + (bias != nullptr ? E::to_f32(bias[n]) : 0.f), act);
-      if (residual != nullptr) z += E::to_f32(residual[m * ldr + n]);
-      out[m * ldo + n] = E::from_f32(z);
+  __device__ __forceinline__ void store(long long m0, const float (&z)[16], const uint16_t (&r)[16]) const {
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+      float2 v = activate(make_float2(z[i] + bias, z[i + 1] + bias), act);
+      if (res != nullptr) {
+        v.x += E::to_f32(*reinterpret_cast<const T*>(&r[i]));
+        v.y += E::to_f32(*reinterpret_cast<const T*>(&r[i + 1]));
+      }
+      if (live && m0 + i < M) out[(m0 + i) * ldo] = E::from_f32(v.x);
+      if (live && m0 + i + 1 < M) out[(m0 + i + 1) * ldo] = E::from_f32(v.y);
     }
+  }
+};
+
+template <typename T, bool PAIR>
+__global__ void __launch_bounds__(kThreads, 1)
+    linear_residual_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a, const LinearParams p) {
+  using E = ElemOps<T>;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    ptx::prefetch_tensor_map(&tm_w);
+    ptx::prefetch_tensor_map(&tm_a);
+  }
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* red = reinterpret_cast<float*>(ring + kRingBytes);
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + kRingBytes + kRedBytes);
+  uint64_t* empty = full + kMaxStages;
+  uint64_t* tfull = empty + kMaxStages;
+  uint64_t* tempty = tfull + 2;
+  uint64_t* drain = tempty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  const bool clustered = PAIR || p.split > 1;
+  const uint32_t rank = clustered ? ptx::cluster_ctarank() : 0;
+  const bool leader = !PAIR || rank == 0;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      ptx::mbar_init(&full[s], 1);
+      ptx::mbar_init(&empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      ptx::mbar_init(&tfull[a], 1);
+      ptx::mbar_init(&tempty[a], (PAIR ? 2 : 1) * kEpiWarps);
+    }
+    ptx::mbar_init(drain, 1);
+    ptx::fence_barrier_init();
+  }
+  if (warp == 1) {
+    if (PAIR) {
+      ptx::tmem_alloc_pair(tmem_slot, 512);
+      ptx::tmem_relinquish_pair();
+    } else {
+      ptx::tmem_alloc(tmem_slot, 512);
+      ptx::tmem_relinquish();
+    }
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (clustered) ptx::cluster_sync();  // every barrier is initialised before a peer signals or writes
+  ptx::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  const long long M = p.rows_dev != nullptr ? min(p.m_cap, (long long)*p.rows_dev) : p.m_cap;
+  const int bt = p.bt;
+  const int num_m = M > 0 ? int((M + bt - 1) / bt) : 0;
+  constexpr int kTileN = PAIR ? 256 : 128;
+  const int num_n = (p.N + kTileN - 1) / kTileN;
+  const long long tiles = (long long)num_m * num_n;
+  const int share = PAIR ? 2 : p.split;  // CTAs that work on one tile
+  const long long first = blockIdx.x / share, stride = gridDim.x / share;
+  // this CTA's K blocks
+  const int kblocks = (p.K + kBK - 1) / kBK;
+  const int kb0 = PAIR ? 0 : int((long long)kblocks * rank / p.split);
+  const int kb1 = PAIR ? kblocks : int((long long)kblocks * (rank + 1) / p.split);
+  const int a_rows = PAIR ? bt / 2 : bt;  // rows of a this CTA loads
+  const int a_atom = a_rows * 128;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      long long issued = 0;
+      bool ok = true;
+      const uint32_t tx = uint32_t(PAIR ? 2 : 1) * uint32_t(kWBytes + 2 * a_atom);
+      for (long long t = first; t < tiles && ok; t += stride) {
+        int nb, mb;
+        tile_at(t, num_n, num_m, nb, mb);
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!(ok = ptx::mbar_wait(&empty[stage], phase ^ 1u, p.err))) break;
+          uint8_t* s_w = ring + stage * p.stage_bytes;
+          uint8_t* s_a = s_w + kWBytes;
+          const int n0 = nb * kTileN + int(PAIR ? rank * 128 : 0), m0 = mb * bt + int(PAIR ? rank * a_rows : 0);
+          if (PAIR) {
+            const uint32_t bar = ptx::mapa_shared(ptx::smem_u32(&full[stage]), 0);
+            if (leader) ptx::mbar_arrive_expect_tx(&full[stage], tx);
+            for (int u = 0; u < 2; ++u) {
+              ptx::tma_load_2d_pair(s_w + u * 16384, &tm_w, kb * kBK + u * 64, n0, bar);
+              ptx::tma_load_2d_pair(s_a + u * a_atom, &tm_a, kb * kBK + u * 64, m0, bar);
+            }
+          } else {
+            ptx::mbar_arrive_expect_tx(&full[stage], tx);
+            for (int u = 0; u < 2; ++u) {
+              ptx::tma_load_2d(s_w + u * 16384, &tm_w, kb * kBK + u * 64, n0, &full[stage]);
+              ptx::tma_load_2d(s_a + u * a_atom, &tm_a, kb * kBK + u * 64, m0, &full[stage]);
+            }
+          }
+          ++issued;
+          if (++stage == p.stages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      // Every slot's last load has landed and been consumed ("empty" again) before the CTA can exit
+      // (bounded; in a pair this is also what keeps the leader's reads of this CTA's slots valid).
+      for (long long j = std::max(0ll, issued - p.stages); j < issued; ++j) {
+        uint64_t* bar = &empty[j % p.stages];
+        const uint32_t parity = uint32_t((j / p.stages) & 1);
+        const unsigned long long t0 = ptx::globaltimer();
+        while (!ptx::mbar_try_wait(bar, parity) && ptx::globaltimer() - t0 < ptx::kTimeoutNs) {
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && leader) {
+      const uint32_t idesc =
+          ptx::idesc_f16_f32(PAIR ? 256 : 128, uint32_t(bt)) | (E::kMmaFormat << 7) | (E::kMmaFormat << 10);
+      int stage = 0, local = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (long long t = first; t < tiles && ok; t += stride, ++local) {
+        const int acc = local & 1;
+        if (!(ok = ptx::mbar_wait(&tempty[acc], ((local >> 1) & 1) ^ 1, p.err))) break;
+        ptx::tc_fence_after();
+        const uint32_t d = tmem + uint32_t(acc * 256);
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!(ok = ptx::mbar_wait(&full[stage], phase, p.err))) break;
+          ptx::tc_fence_after();
+          const uint32_t w_addr = ptx::smem_u32(ring + stage * p.stage_bytes), a_addr = w_addr + kWBytes;
+#pragma unroll
+          for (int k = 0; k < kBK / 16; ++k) {
+            const uint64_t dw = ptx::desc_kmajor_sw128(w_addr + (k >> 2) * 16384 + (k & 3) * 32);
+            const uint64_t da = ptx::desc_kmajor_sw128(a_addr + (k >> 2) * a_atom + (k & 3) * 32);
+            if (PAIR)
+              ptx::umma_f16_ss_pair(d, dw, da, idesc, (kb != kb0) | (k != 0));
+            else
+              ptx::umma_f16_ss(d, dw, da, idesc, (kb != kb0) | (k != 0));
+          }
+          if (PAIR)
+            ptx::umma_commit_pair_mc(&empty[stage], 0x3);
+          else
+            ptx::umma_commit(&empty[stage]);
+          if (++stage == p.stages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+        if (PAIR)
+          ptx::umma_commit_pair_mc(&tfull[acc], 0x3);
+        else
+          ptx::umma_commit(&tfull[acc]);
+      }
+      // every issued MMA is done before TMEM is released
+      if (PAIR)
+        ptx::umma_commit_pair(ptx::mapa_shared(ptx::smem_u32(drain), 0));
+      else
+        ptx::umma_commit(drain);
+      const unsigned long long t0 = ptx::globaltimer();
+      while (!ptx::mbar_try_wait(drain, 0) && ptx::globaltimer() - t0 < ptx::kTimeoutNs) {
+      }
+    }
+    __syncwarp();
+  } else {
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    int local = 0;
+    for (long long t = first; t < tiles; t += stride, ++local) {
+      const int acc = local & 1;
+      int nb, mb;
+      tile_at(t, num_n, num_m, nb, mb);
+      const int n = nb * kTileN + int(PAIR ? rank * 128 : 0) + quarter * 32 + lane;
+      Column<T> col{static_cast<const T*>(p.residual), static_cast<T*>(p.out), p.ldr, p.ldo, M, 0.f, p.act, n < p.N};
+      if (col.res != nullptr) col.res += n;
+      col.out += n;
+      if (p.bias != nullptr && col.live) col.bias = E::to_f32(static_cast<const T*>(p.bias)[n]);
+      const long long m_tile = (long long)mb * bt;
+      const uint32_t t_row = tmem + (uint32_t(quarter * 32) << 16) + uint32_t(acc * 256);
+      const int chunks = bt / 16;
+      if (!PAIR && p.split > 1) {
+        // this share's sums to the CTA that finishes each column: red[source][column of its share][lane]
+        if (!__all_sync(0xffffffffu, ptx::mbar_wait(&tfull[acc], 0, p.err))) break;
+        ptx::tc_fence_after();
+        const int mine = bt / p.split;  // columns each CTA finishes
+        for (int c = half; c < chunks; c += 2) {
+          uint32_t z[16];
+          ptx::tmem_ld_32x32b_x16(t_row + c * 16, z);
+          ptx::tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int column = c * 16 + i;
+            const uint32_t dst = ptx::mapa_shared(
+                ptx::smem_u32(red + (int(rank) * mine + column % mine) * 128 + quarter * 32 + lane), uint32_t(column / mine));
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(__uint_as_float(z[i])) : "memory");
+          }
+        }
+        break;  // one tile a cluster; finished below
+      }
+      uint16_t r[2][16];
+      col.fetch(m_tile + half * 16, r[0]);
+      if (!__all_sync(0xffffffffu, ptx::mbar_wait(&tfull[acc], (local >> 1) & 1, p.err))) break;
+      ptx::tc_fence_after();
+      for (int c = half; c < chunks; c += 4) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {  // the residuals of the next chunk are on their way during this one
+          const int cc = c + 2 * u;
+          if (cc < chunks) {
+            uint32_t z[16];
+            ptx::tmem_ld_32x32b_x16(t_row + cc * 16, z);
+            if (cc + 2 < chunks) col.fetch(m_tile + (cc + 2) * 16, r[u ^ 1]);
+            ptx::tmem_wait_ld();
+            float zf[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) zf[i] = __uint_as_float(z[i]);
+            col.store(m_tile + cc * 16, zf, r[u]);
+          }
+        }
+      }
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (PAIR)
+          ptx::mbar_arrive_cluster(ptx::mapa_shared(ptx::smem_u32(&tempty[acc]), 0));
+        else
+          ptx::mbar_arrive(&tempty[acc]);
+      }
+    }
+  }
+  __syncwarp();
+  if (!PAIR && p.split > 1) {
+    ptx::cluster_sync();  // all shares' sums have arrived
+    if (warp >= 2 && first < tiles) {
+      const int quarter = warp & 3, half = (warp - 2) >> 2;
+      int nb, mb;
+      tile_at(first, num_n, num_m, nb, mb);
+      const int n = nb * 128 + quarter * 32 + lane, mine = bt / p.split;
+      const bool live = n < p.N;
+      const T* res = static_cast<const T*>(p.residual);
+      T* out = static_cast<T*>(p.out);
+      const float bias = p.bias != nullptr && live ? E::to_f32(static_cast<const T*>(p.bias)[n]) : 0.f;
+      for (int j = half; j < mine; j += 2) {
+        const long long m = (long long)mb * bt + int(rank) * mine + j;
+        if (!live || m >= M) continue;
+        float z = 0.f;
+        for (int s = 0; s < p.split; ++s) z += red[(s * mine + j) * 128 + quarter * 32 + lane];
+        z = activate(make_float2(z + bias, 0.f), p.act).x;
+        if (res != nullptr) z += E::to_f32(res[m * p.ldr + n]);
+        out[m * p.ldo + n] = E::from_f32(z);
+      }
+    }
+  }
+
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (PAIR) ptx::cluster_sync();  // neither CTA leaves while the pair may still touch its memory
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    if (PAIR)
+      ptx::tmem_dealloc_pair(tmem, 512);
+    else
+      ptx::tmem_dealloc(tmem, 512);
+  }
+}
+
+// ------------------------------------------------------------------------------------- host
+
+gdc_status encode(CUtensorMap* map, bool bf16, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows) {
+  auto fn = get_encode_fn();
+  if (!fn) return set_error(GDC_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  const cuuint64_t dims[2] = {cols, rows}, strides[1] = {ld * 2};
+  const cuuint32_t box[2] = {64, box_rows}, estr[2] = {1, 1};
+  const CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims,
+                        strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(GDC_ERR_CUDA, "cuTensorMapEncodeTiled (linear residual) failed (%d)", int(r));
+  return GDC_OK;
+}
+
+struct Config {
+  bool pair;
+  int bt, split;
+};
+
+// The form of a call: the estimated time (in tensor-core cycles) of every form is its rounds over
+// the SMs times a tile's time; the least wins.
+Config choose(int64_t M, int N, int K, int sms) {
+  Config best{false, 16, 1};
+  double best_cost = 1e300;
+  const double kblocks = double((K + kBK - 1) / kBK);
+  auto consider = [&](const Config& c) {
+    const int64_t tile_n = c.pair ? 256 : 128;
+    const int64_t tiles = ((N + tile_n - 1) / tile_n) * ((M + c.bt - 1) / c.bt);
+    const int64_t ctas = tiles * (c.pair ? 2 : c.split);
+    if (c.split > 1 && ctas > sms) return;
+    const double rounds = double(c.pair ? (tiles + sms / 2 - 1) / (sms / 2) : (ctas + sms - 1) / sms);
+    // a K block: the MMA's own cycles (8 of K = 16, bt / 2 cycles each), or the shared-memory traffic of its
+    // operands where that is more
+    const double a_rows = c.pair ? c.bt / 2 : c.bt;
+    const double block = std::max(4.0 * c.bt, (128 + a_rows) * kBK * 2 * 2 / 128.0);
+    const double cost = rounds * (kblocks / c.split * block + 300) + (c.split > 1 ? 600 : 0) + 8.0 * c.bt;
+    if (cost < best_cost * 0.999) {
+      best_cost = cost;
+      best = c;
+    }
+  };
+  const int bt_max = int(std::min<int64_t>(256, (M + 15) / 16 * 16));
+  for (int bt = bt_max; bt >= 16; bt -= 16) {
+    if (M > 128 && bt >= 32) consider({true, bt, 1});
+    consider({false, bt, 1});
+    if (bt <= kMaxSplitBt)
+      for (int s = 2; s <= 8; s *= 2)
+        if (s <= int(kblocks)) consider({false, bt, s});
+  }
+  return best;
+}
+
+template <typename T, bool PAIR>
+gdc_status launch_form(const CUtensorMap& tw, const CUtensorMap& ta, const LinearParams& p, int grid, int cluster, cudaStream_t stream,
+                       int dev) {
+  auto kern = linear_residual_kernel<T, PAIR>;
+  static PerDeviceOnce configured;
+  const cudaError_t ce = cudaError_t(per_device_once(
+      configured, dev, [&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes); }));
+  if (ce != cudaSuccess) return set_error(GDC_ERR_CUDA, "linear residual smem attribute: %s", cudaGetErrorString(ce));
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = unsigned(cluster);
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(grid));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmemBytes;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  GDC_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, tw, ta, p));
+  return GDC_OK;
 }
 
 template <typename T>
-gdc_status launch_typed(const LinearResidualArgs& p, cudaStream_t stream) {
-  const dim3 grid(unsigned((p.M + kTile - 1) / kTile), unsigned((p.N + kTile - 1) / kTile));
-  if (grid.y > 65535) return set_error(GDC_ERR_UNSUPPORTED, "gdc_linear_residual: N=%d too large", p.N);
-  linear_residual_kernel<T><<<grid, 256, 0, stream>>>(
-      static_cast<const T*>(p.a), static_cast<const T*>(p.w), static_cast<const T*>(p.bias),
-      static_cast<const T*>(p.residual), static_cast<T*>(p.out), p.lda, p.ldw, p.ldr, p.ldo, p.M, p.rows_dev, p.N, p.K,
-      p.act);
-  return check_launch("linear_residual_kernel");
+gdc_status launch_typed(const LinearResidualArgs& a, cudaStream_t stream, int* err) {
+  constexpr bool bf16 = ElemOps<T>::kMmaFormat == 1;
+  int dev = 0;
+  GDC_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64) return set_error(GDC_ERR_CUDA, "device ordinal out of range");
+  const int sms = device_sm_count(dev);
+  const Config c = choose(a.M, a.N, a.K, sms);
+  const int a_rows = c.pair ? c.bt / 2 : c.bt;
+  CUtensorMap tw, ta;
+  GDC_TRY(encode(&tw, bf16, a.w, uint64_t(a.N), uint64_t(a.K), uint64_t(a.ldw), 128));
+  GDC_TRY(encode(&ta, bf16, a.a, uint64_t(a.M), uint64_t(a.K), uint64_t(a.lda), uint32_t(a_rows)));
+  LinearParams p{};
+  p.bias = a.bias;
+  p.residual = a.residual;
+  p.out = a.out;
+  p.ldr = a.ldr;
+  p.ldo = a.ldo;
+  p.m_cap = a.M;
+  p.rows_dev = a.rows_dev;
+  p.N = a.N;
+  p.K = a.K;
+  p.act = a.act;
+  p.bt = c.bt;
+  p.split = c.split;
+  p.stage_bytes = kWBytes + a_rows * kBK * 2;
+  p.stages = std::min(kMaxStages, kRingBytes / p.stage_bytes);
+  p.err = err;
+  const int64_t tile_n = c.pair ? 256 : 128;
+  const int64_t tiles = ((a.N + tile_n - 1) / tile_n) * ((a.M + c.bt - 1) / c.bt);
+  if (c.pair) return launch_form<T, true>(tw, ta, p, 2 * int(std::min<int64_t>(tiles, sms / 2)), 2, stream, dev);
+  const int grid = c.split > 1 ? int(tiles * c.split) : int(std::min<int64_t>(tiles, sms));
+  return launch_form<T, false>(tw, ta, p, grid, c.split, stream, dev);
 }
 
 }  // namespace
 
-gdc_status launch_linear_residual(Elem t, const LinearResidualArgs& a, cudaStream_t stream, int*) {
-  return t == Elem::kF16 ? launch_typed<__half>(a, stream) : launch_typed<__nv_bfloat16>(a, stream);
+gdc_status launch_linear_residual(Elem t, const LinearResidualArgs& a, cudaStream_t stream, int* err) {
+  return t == Elem::kF16 ? launch_typed<__half>(a, stream, err) : launch_typed<__nv_bfloat16>(a, stream, err);
 }
 
 }  // namespace gdc
