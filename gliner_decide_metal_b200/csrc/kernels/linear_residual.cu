@@ -16,8 +16,10 @@
 //           splits K, and each sums its share of the columns from all of them, in rank order,
 //           through distributed shared memory.
 //
-// Roles: warp 0 TMA (128-column K blocks of w and a into a ring), warp 1 MMA issue, warps 2-9
-// epilogue (TMEM lane quarter warp % 4; two warps a quarter take alternate 16-column chunks).
+// Roles: warp 0 TMA (128-column K blocks of w and a into a ring), warp 1 MMA issue, warps 2-17
+// epilogue (TMEM lane quarter warp % 4; the four warps of a quarter take 16-column chunks in turn).
+// An epilogue warp has the residuals of its whole tile share (up to 64 rows, 64 bytes each) on
+// their way before it waits for the accumulators.
 // Sums are fp32 over K in order (K split: in order inside a share, shares in rank order): the
 // same call gives the same bits.
 #include <cuda.h>
@@ -37,7 +39,7 @@ PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn();
 namespace {
 
 constexpr int kBK = 128;         // K columns of a stage: two 128-byte swizzle atoms an operand
-constexpr int kEpiWarps = 8;
+constexpr int kEpiWarps = 16;    // four a TMEM lane quarter, each every fourth 16-column chunk
 constexpr int kThreads = 64 + 32 * kEpiWarps;
 constexpr int kMaxStages = 6;
 constexpr int kWBytes = 128 * kBK * 2;
@@ -51,7 +53,7 @@ struct LinearParams {
   void* out;
   long long ldr, ldo, m_cap;
   const int32_t* rows_dev;
-  int N, K, act, bt, split, stages, stage_bytes;
+  int N, K, bt, split, stages, stage_bytes;
   int* err;
 };
 
@@ -66,53 +68,69 @@ __device__ __forceinline__ void tile_at(long long t, int num_n, int num_m, int& 
 }
 
 // The activation of two values (rows m, m + 1 of one n).
-__device__ __forceinline__ float2 activate(float2 z, int act) {
-  if (act == kActGelu) {
+template <int ACT>
+__device__ __forceinline__ float2 activate(float2 z) {
+  if (ACT == kActGelu) {
     const float2 g = gelu_erf2(z);
     return make_float2(z.x > 16.f ? z.x : g.x, z.y > 16.f ? z.y : g.y);  // GELU(x) = x there; keeps +inf
   }
-  if (act == kActRelu) {
+  if (ACT == kActRelu) {
     asm("max.NaN.f32 %0, %0, 0f00000000;" : "+f"(z.x));
     asm("max.NaN.f32 %0, %0, 0f00000000;" : "+f"(z.y));
-    return z;
   }
-  if (act == kActSilu)
+  if (ACT == kActSilu)
     return make_float2(__fdividef(z.x, 1.f + ex2_approx_f32(-kGeluLog2e * z.x)),
                        __fdividef(z.y, 1.f + ex2_approx_f32(-kGeluLog2e * z.y)));
   return z;
 }
 
-// One chunk of 16 rows m0.. of column n: residuals are fetched ahead (fetch), then joined with the
-// accumulators and stored.
-template <typename T>
+// Column n of the outputs: rows are fetched and stored 16 at a time.
+template <typename T, int ACT>
 struct Column {
   using E = ElemOps<T>;
   const T* res;
   T* out;
   long long ldr, ldo, M;
   float bias;
-  int act;
-  bool live;
+  // residuals of rows m0 .. m0 + 15 (those outside the matrix stay unset)
   __device__ __forceinline__ void fetch(long long m0, uint16_t (&r)[16]) const {
+    const uint16_t* src = reinterpret_cast<const uint16_t*>(res) + m0 * ldr;
+    if (m0 + 16 <= M) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      r[i] = res != nullptr && live && m0 + i < M ? *reinterpret_cast<const uint16_t*>(res + (m0 + i) * ldr) : uint16_t(0);
+      for (int i = 0; i < 16; ++i, src += ldr) r[i] = *src;
+    } else {
+      const int rows = int(max(0ll, M - m0));
+#pragma unroll
+      for (int i = 0; i < 16; ++i, src += ldr)
+        if (i < rows) r[i] = *src;
+    }
   }
-  __device__ __forceinline__ void store(long long m0, const float (&z)[16], const uint16_t (&r)[16]) const {
+  __device__ __forceinline__ void store(long long m0, const uint32_t (&z)[16], const uint16_t (&r)[16]) const {
+    float v[16];
 #pragma unroll
     for (int i = 0; i < 16; i += 2) {
-      float2 v = activate(make_float2(z[i] + bias, z[i + 1] + bias), act);
-      if (res != nullptr) {
-        v.x += E::to_f32(*reinterpret_cast<const T*>(&r[i]));
-        v.y += E::to_f32(*reinterpret_cast<const T*>(&r[i + 1]));
-      }
-      if (live && m0 + i < M) out[(m0 + i) * ldo] = E::from_f32(v.x);
-      if (live && m0 + i + 1 < M) out[(m0 + i + 1) * ldo] = E::from_f32(v.y);
+      const float2 x = activate<ACT>(__fadd2_rn(make_float2(__uint_as_float(z[i]), __uint_as_float(z[i + 1])), make_float2(bias, bias)));
+      v[i] = x.x;
+      v[i + 1] = x.y;
+    }
+    if (res != nullptr) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] += E::to_f32(*reinterpret_cast<const T*>(&r[i]));
+    }
+    T* dst = out + m0 * ldo;
+    if (m0 + 16 <= M) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i, dst += ldo) *dst = E::from_f32(v[i]);
+    } else {
+      const int rows = int(max(0ll, M - m0));
+#pragma unroll
+      for (int i = 0; i < 16; ++i, dst += ldo)
+        if (i < rows) *dst = E::from_f32(v[i]);
     }
   }
 };
 
-template <typename T, bool PAIR>
+template <typename T, bool PAIR, int ACT>
 __global__ void __launch_bounds__(kThreads, 1)
     linear_residual_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a, const LinearParams p) {
   using E = ElemOps<T>;
@@ -273,17 +291,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
   } else {
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const int quarter = warp & 3, part = (warp - 2) >> 2;
     int local = 0;
     for (long long t = first; t < tiles; t += stride, ++local) {
       const int acc = local & 1;
       int nb, mb;
       tile_at(t, num_n, num_m, nb, mb);
       const int n = nb * kTileN + int(PAIR ? rank * 128 : 0) + quarter * 32 + lane;
-      Column<T> col{static_cast<const T*>(p.residual), static_cast<T*>(p.out), p.ldr, p.ldo, M, 0.f, p.act, n < p.N};
+      const bool live = n < p.N;
+      Column<T, ACT> col{static_cast<const T*>(p.residual), static_cast<T*>(p.out) + n, p.ldr, p.ldo, M, 0.f};
       if (col.res != nullptr) col.res += n;
-      col.out += n;
-      if (p.bias != nullptr && col.live) col.bias = E::to_f32(static_cast<const T*>(p.bias)[n]);
+      if (p.bias != nullptr && live) col.bias = E::to_f32(static_cast<const T*>(p.bias)[n]);
       const long long m_tile = (long long)mb * bt;
       const uint32_t t_row = tmem + (uint32_t(quarter * 32) << 16) + uint32_t(acc * 256);
       const int chunks = bt / 16;
@@ -292,7 +310,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!__all_sync(0xffffffffu, ptx::mbar_wait(&tfull[acc], 0, p.err))) break;
         ptx::tc_fence_after();
         const int mine = bt / p.split;  // columns each CTA finishes
-        for (int c = half; c < chunks; c += 2) {
+        for (int c = part; c < chunks; c += 4) {
           uint32_t z[16];
           ptx::tmem_ld_32x32b_x16(t_row + c * 16, z);
           ptx::tmem_wait_ld();
@@ -306,24 +324,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         break;  // one tile a cluster; finished below
       }
-      uint16_t r[2][16];
-      col.fetch(m_tile + half * 16, r[0]);
+      uint16_t r[4][16];
+      if (col.res != nullptr && live) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (part + 4 * u < chunks) col.fetch(m_tile + (part + 4 * u) * 16, r[u]);
+      }
       if (!__all_sync(0xffffffffu, ptx::mbar_wait(&tfull[acc], (local >> 1) & 1, p.err))) break;
       ptx::tc_fence_after();
-      for (int c = half; c < chunks; c += 4) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {  // the residuals of the next chunk are on their way during this one
-          const int cc = c + 2 * u;
-          if (cc < chunks) {
-            uint32_t z[16];
-            ptx::tmem_ld_32x32b_x16(t_row + cc * 16, z);
-            if (cc + 2 < chunks) col.fetch(m_tile + (cc + 2) * 16, r[u ^ 1]);
-            ptx::tmem_wait_ld();
-            float zf[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) zf[i] = __uint_as_float(z[i]);
-            col.store(m_tile + cc * 16, zf, r[u]);
-          }
+      for (int u = 0; u < 4; ++u) {
+        const int c = part + 4 * u;
+        if (c < chunks) {
+          uint32_t z[16];
+          ptx::tmem_ld_32x32b_x16(t_row + c * 16, z);
+          ptx::tmem_wait_ld();
+          if (live) col.store(m_tile + c * 16, z, r[u]);
         }
       }
       ptx::tc_fence_before();
@@ -340,7 +356,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (!PAIR && p.split > 1) {
     ptx::cluster_sync();  // all shares' sums have arrived
     if (warp >= 2 && first < tiles) {
-      const int quarter = warp & 3, half = (warp - 2) >> 2;
+      const int quarter = warp & 3, part = (warp - 2) >> 2;
       int nb, mb;
       tile_at(first, num_n, num_m, nb, mb);
       const int n = nb * 128 + quarter * 32 + lane, mine = bt / p.split;
@@ -348,12 +364,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       const T* res = static_cast<const T*>(p.residual);
       T* out = static_cast<T*>(p.out);
       const float bias = p.bias != nullptr && live ? E::to_f32(static_cast<const T*>(p.bias)[n]) : 0.f;
-      for (int j = half; j < mine; j += 2) {
+      for (int j = part; j < mine; j += 4) {
         const long long m = (long long)mb * bt + int(rank) * mine + j;
         if (!live || m >= M) continue;
         float z = 0.f;
         for (int s = 0; s < p.split; ++s) z += red[(s * mine + j) * 128 + quarter * 32 + lane];
-        z = activate(make_float2(z + bias, 0.f), p.act).x;
+        z = activate<ACT>(make_float2(z + bias, 0.f)).x;
         if (res != nullptr) z += E::to_f32(res[m * p.ldr + n]);
         out[m * p.ldo + n] = E::from_f32(z);
       }
@@ -424,10 +440,10 @@ Config choose(int64_t M, int N, int K, int sms) {
   return best;
 }
 
-template <typename T, bool PAIR>
+template <typename T, bool PAIR, int ACT>
 gdc_status launch_form(const CUtensorMap& tw, const CUtensorMap& ta, const LinearParams& p, int grid, int cluster, cudaStream_t stream,
                        int dev) {
-  auto kern = linear_residual_kernel<T, PAIR>;
+  auto kern = linear_residual_kernel<T, PAIR, ACT>;
   static PerDeviceOnce configured;
   const cudaError_t ce = cudaError_t(per_device_once(
       configured, dev, [&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes); }));
@@ -469,7 +485,6 @@ gdc_status launch_typed(const LinearResidualArgs& a, cudaStream_t stream, int* e
   p.rows_dev = a.rows_dev;
   p.N = a.N;
   p.K = a.K;
-  p.act = a.act;
   p.bt = c.bt;
   p.split = c.split;
   p.stage_bytes = kWBytes + a_rows * kBK * 2;
@@ -477,9 +492,19 @@ gdc_status launch_typed(const LinearResidualArgs& a, cudaStream_t stream, int* e
   p.err = err;
   const int64_t tile_n = c.pair ? 256 : 128;
   const int64_t tiles = ((a.N + tile_n - 1) / tile_n) * ((a.M + c.bt - 1) / c.bt);
-  if (c.pair) return launch_form<T, true>(tw, ta, p, 2 * int(std::min<int64_t>(tiles, sms / 2)), 2, stream, dev);
-  const int grid = c.split > 1 ? int(tiles * c.split) : int(std::min<int64_t>(tiles, sms));
-  return launch_form<T, false>(tw, ta, p, grid, c.split, stream, dev);
+  const int cluster = c.pair ? 2 : c.split;
+  const int grid = c.pair ? 2 * int(std::min<int64_t>(tiles, sms / 2))
+                          : (c.split > 1 ? int(tiles * c.split) : int(std::min<int64_t>(tiles, sms)));
+  switch (a.act * 2 + c.pair) {
+    case 2 * kActNone: return launch_form<T, false, kActNone>(tw, ta, p, grid, cluster, stream, dev);
+    case 2 * kActNone + 1: return launch_form<T, true, kActNone>(tw, ta, p, grid, cluster, stream, dev);
+    case 2 * kActGelu: return launch_form<T, false, kActGelu>(tw, ta, p, grid, cluster, stream, dev);
+    case 2 * kActGelu + 1: return launch_form<T, true, kActGelu>(tw, ta, p, grid, cluster, stream, dev);
+    case 2 * kActRelu: return launch_form<T, false, kActRelu>(tw, ta, p, grid, cluster, stream, dev);
+    case 2 * kActRelu + 1: return launch_form<T, true, kActRelu>(tw, ta, p, grid, cluster, stream, dev);
+    case 2 * kActSilu: return launch_form<T, false, kActSilu>(tw, ta, p, grid, cluster, stream, dev);
+    default: return launch_form<T, true, kActSilu>(tw, ta, p, grid, cluster, stream, dev);
+  }
 }
 
 }  // namespace
