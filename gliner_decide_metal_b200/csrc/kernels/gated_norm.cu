@@ -119,6 +119,8 @@ __global__ void __launch_bounds__(512)
                       long long gate_rows, const int32_t* __restrict__ gate_index, const int32_t* __restrict__ rows_dev,
                       int post, int pre, int cols, float scale, float eps, int tpr, int* err) {
   __shared__ float red[64];
+  ptx::grid_launch_next();
+  ptx::grid_wait();
   const int in_row = threadIdx.x & (tpr - 1);
   const int rows_per_block = blockDim.x / tpr;
   const long long row = (long long)blockIdx.x * rows_per_block + threadIdx.x / tpr;
@@ -182,12 +184,12 @@ gdc_status launch_variant(const GatedNormArgs& a, int tpr, cudaStream_t stream, 
   const int threads = tpr > kThreads ? tpr : kThreads;
   const int per_block = threads / tpr;
   const long long blocks = (a.rows + per_block - 1) / per_block;
-  gated_norm_kernel<T, VEC, CH><<<unsigned(blocks), threads, 0, stream>>>(
-      static_cast<const T*>(a.y), static_cast<const T*>(a.x), static_cast<const T*>(a.post_w),
-      static_cast<const T*>(a.post_b), static_cast<const T*>(a.gate), static_cast<const T*>(a.pre_w),
-      static_cast<const T*>(a.pre_b), static_cast<T*>(a.x_out), static_cast<T*>(a.n_out), a.ldy, a.ldx, a.ldxo, a.ldno,
-      a.rows, a.gate_rows, a.gate_index, a.rows_dev, a.post, a.pre, a.cols, a.scale, a.eps, tpr, err);
-  return check_launch("gated_norm_kernel");
+  GDC_CUDA_TRY(launch_overlapped(
+      gated_norm_kernel<T, VEC, CH>, unsigned(blocks), unsigned(threads), 0, 1, stream, static_cast<const T*>(a.y),
+      static_cast<const T*>(a.x), static_cast<const T*>(a.post_w), static_cast<const T*>(a.post_b), static_cast<const T*>(a.gate),
+      static_cast<const T*>(a.pre_w), static_cast<const T*>(a.pre_b), static_cast<T*>(a.x_out), static_cast<T*>(a.n_out), a.ldy, a.ldx,
+      a.ldxo, a.ldno, a.rows, a.gate_rows, a.gate_index, a.rows_dev, a.post, a.pre, a.cols, a.scale, a.eps, tpr, err));
+  return GDC_OK;
 }
 
 template <typename T>

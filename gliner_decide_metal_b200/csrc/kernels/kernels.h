@@ -103,6 +103,28 @@ gdc_status launch_decode(const float* logits, int batch, int max_heads, int max_
 
 // ---- block operators over packed rows (arguments already checked by block_api.cpp) ----
 
+// Launches a kernel of the block operators, in clusters of `cluster` CTAs, with programmatic
+// stream serialisation: its set-up may overlap the end of the kernel before it, whose results it
+// waits for itself (ptx::grid_wait).
+template <typename... KArgs, typename... Args>
+cudaError_t launch_overlapped(void (*kern)(KArgs...), unsigned grid, unsigned threads, size_t smem, unsigned cluster,
+                              cudaStream_t stream, const Args&... args) {
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, KArgs(args)...);
+}
+
 // Element type of a block operator's tensors.
 enum class Elem : int { kF16 = 0, kBF16 = 1 };
 

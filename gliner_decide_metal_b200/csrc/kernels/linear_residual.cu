@@ -44,9 +44,10 @@ constexpr int kThreads = 64 + 32 * kEpiWarps;
 constexpr int kMaxStages = 6;
 constexpr int kWBytes = 128 * kBK * 2;
 constexpr int kRingBytes = 192 * 1024;
+constexpr int kSmallRing = 108 * 1024;  // leaves room for a second CTA's set-up on the SM
 constexpr int kMaxSplitBt = 64;  // split K: columns x 128 lanes x 4 bytes of partial sums, 32 KB
-constexpr int kRedBytes = kMaxSplitBt * 512;
-constexpr int kSmemBytes = kRingBytes + kRedBytes + 1024 + 256;
+constexpr int kCtrlBytes = 256;
+constexpr int kMaxSmem = kRingBytes + kMaxSplitBt * 512 + kCtrlBytes + 1024;
 
 struct LinearParams {
   const void *bias, *residual;
@@ -54,6 +55,7 @@ struct LinearParams {
   long long ldr, ldo, m_cap;
   const int32_t* rows_dev;
   int N, K, bt, split, stages, stage_bytes;
+  int acc_cols, tmem_cols;  // TMEM columns between accumulators, and in all
   int* err;
 };
 
@@ -135,14 +137,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     linear_residual_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a, const LinearParams p) {
   using E = ElemOps<T>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  ptx::grid_launch_next();
   if (threadIdx.x == 0) {
     ptx::prefetch_tensor_map(&tm_w);
     ptx::prefetch_tensor_map(&tm_a);
   }
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* red = reinterpret_cast<float*>(ring + kRingBytes);
-  uint64_t* full = reinterpret_cast<uint64_t*>(ring + kRingBytes + kRedBytes);
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + p.stages * p.stage_bytes);
+  float* red = reinterpret_cast<float*>(ring + p.stages * p.stage_bytes + kCtrlBytes);
   uint64_t* empty = full + kMaxStages;
   uint64_t* tfull = empty + kMaxStages;
   uint64_t* tempty = tfull + 2;
@@ -166,10 +169,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   if (warp == 1) {
     if (PAIR) {
-      ptx::tmem_alloc_pair(tmem_slot, 512);
+      ptx::tmem_alloc_pair(tmem_slot, p.tmem_cols);
       ptx::tmem_relinquish_pair();
     } else {
-      ptx::tmem_alloc(tmem_slot, 512);
+      ptx::tmem_alloc(tmem_slot, p.tmem_cols);
       ptx::tmem_relinquish();
     }
   }
@@ -178,6 +181,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (clustered) ptx::cluster_sync();  // every barrier is initialised before a peer signals or writes
   ptx::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  ptx::grid_wait();
 
   const long long M = p.rows_dev != nullptr ? min(p.m_cap, (long long)*p.rows_dev) : p.m_cap;
   const int bt = p.bt;
@@ -251,7 +255,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int acc = local & 1;
         if (!(ok = ptx::mbar_wait(&tempty[acc], ((local >> 1) & 1) ^ 1, p.err))) break;
         ptx::tc_fence_after();
-        const uint32_t d = tmem + uint32_t(acc * 256);
+        const uint32_t d = tmem + uint32_t(acc * p.acc_cols);
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!(ok = ptx::mbar_wait(&full[stage], phase, p.err))) break;
           ptx::tc_fence_after();
@@ -303,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (col.res != nullptr) col.res += n;
       if (p.bias != nullptr && live) col.bias = E::to_f32(static_cast<const T*>(p.bias)[n]);
       const long long m_tile = (long long)mb * bt;
-      const uint32_t t_row = tmem + (uint32_t(quarter * 32) << 16) + uint32_t(acc * 256);
+      const uint32_t t_row = tmem + (uint32_t(quarter * 32) << 16) + uint32_t(acc * p.acc_cols);
       const int chunks = bt / 16;
       if (!PAIR && p.split > 1) {
         // this share's sums to the CTA that finishes each column: red[source][column of its share][lane]
@@ -324,10 +328,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         break;  // one tile a cluster; finished below
       }
-      uint16_t r[4][16];
+      uint16_t r[3][16];
       if (col.res != nullptr && live) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < 3; ++u)
           if (part + 4 * u < chunks) col.fetch(m_tile + (part + 4 * u) * 16, r[u]);
       }
       if (!__all_sync(0xffffffffu, ptx::mbar_wait(&tfull[acc], (local >> 1) & 1, p.err))) break;
@@ -339,7 +343,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t z[16];
           ptx::tmem_ld_32x32b_x16(t_row + c * 16, z);
           ptx::tmem_wait_ld();
-          if (live) col.store(m_tile + c * 16, z, r[u]);
+          if (live) col.store(m_tile + c * 16, z, r[u % 3]);
+          if (u == 0 && col.res != nullptr && live && part + 12 < chunks) col.fetch(m_tile + (part + 12) * 16, r[0]);
         }
       }
       ptx::tc_fence_before();
@@ -382,9 +387,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 1) {
     ptx::tc_fence_after();
     if (PAIR)
-      ptx::tmem_dealloc_pair(tmem, 512);
+      ptx::tmem_dealloc_pair(tmem, p.tmem_cols);
     else
-      ptx::tmem_dealloc(tmem, 512);
+      ptx::tmem_dealloc(tmem, p.tmem_cols);
   }
 }
 
@@ -446,20 +451,10 @@ gdc_status launch_form(const CUtensorMap& tw, const CUtensorMap& ta, const Linea
   auto kern = linear_residual_kernel<T, PAIR, ACT>;
   static PerDeviceOnce configured;
   const cudaError_t ce = cudaError_t(per_device_once(
-      configured, dev, [&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes); }));
+      configured, dev, [&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem); }));
   if (ce != cudaSuccess) return set_error(GDC_ERR_CUDA, "linear residual smem attribute: %s", cudaGetErrorString(ce));
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = unsigned(cluster);
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(grid));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = kSmemBytes;
-  cfg.stream = stream;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  GDC_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, tw, ta, p));
+  const size_t smem = size_t(p.stages) * p.stage_bytes + kCtrlBytes + 1024 + (p.split > 1 ? size_t(p.bt) * 512 : 0);
+  GDC_CUDA_TRY(launch_overlapped(kern, unsigned(grid), kThreads, smem, unsigned(cluster), stream, tw, ta, p));
   return GDC_OK;
 }
 
@@ -488,10 +483,17 @@ gdc_status launch_typed(const LinearResidualArgs& a, cudaStream_t stream, int* e
   p.bt = c.bt;
   p.split = c.split;
   p.stage_bytes = kWBytes + a_rows * kBK * 2;
-  p.stages = std::min(kMaxStages, kRingBytes / p.stage_bytes);
-  p.err = err;
+  // A call of one round keeps to a small ring and little TMEM, so that the next kernel's set-up can
+  // run beside it; more rounds use the SM's whole shared memory.
   const int64_t tile_n = c.pair ? 256 : 128;
   const int64_t tiles = ((a.N + tile_n - 1) / tile_n) * ((a.M + c.bt - 1) / c.bt);
+  const bool small = tiles * (c.pair ? 2 : c.split) <= sms;
+  p.stages = std::min(kMaxStages, (small ? kSmallRing : kRingBytes) / p.stage_bytes);
+  if (p.stages < 2) p.stages = kRingBytes / p.stage_bytes;
+  p.acc_cols = (c.bt + 31) / 32 * 32;
+  p.tmem_cols = 32;
+  while (p.tmem_cols < (small ? 1 : 2) * p.acc_cols) p.tmem_cols *= 2;
+  p.err = err;
   const int cluster = c.pair ? 2 : c.split;
   const int grid = c.pair ? 2 * int(std::min<int64_t>(tiles, sms / 2))
                           : (c.split > 1 ? int(tiles * c.split) : int(std::min<int64_t>(tiles, sms)));

@@ -202,9 +202,6 @@ __device__ void store_row_by_definition(const Params& p, int q_row, int lq, int 
   for (int i = 0; i < PER / 2; ++i) dst[i] = E::pack(o[2 * i], o[2 * i + 1]);
 }
 
-__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
 // ------------------------------------------------------------------------------------- plan
 
 constexpr int kBuckets = 512;
@@ -215,7 +212,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(Params p) {
   __shared__ int hist[kBuckets];
   __shared__ unsigned long long s_work;
   __shared__ int s_items, s_max, s_slots, s_splits;
-  pdl_launch();
+  ptx::grid_launch_next();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = kPlanThreads / 32;
   const int per_item = 2 * p.tile_pos;
   if (threadIdx.x == 0) {
@@ -223,6 +220,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(Params p) {
     s_items = s_max = s_slots = s_splits = 0;
   }
   for (int i = threadIdx.x; i < kBuckets; i += kPlanThreads) hist[i] = 0;
+  ptx::grid_wait();
   __syncthreads();
   auto tiles_of = [&](int pos, int lq, int lk) {
     return (seen_keys(min(pos + per_item, lq) - 1, lq, lk, p.causal) + kKeys - 1) / kKeys;
@@ -442,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int* err = p.err;
 
-  if (PLANNED) pdl_launch();
+  ptx::grid_launch_next();
   if (threadIdx.x == 0) {
     ptx::prefetch_tensor_map(&tm_q);
     ptx::prefetch_tensor_map(&tm_k);
@@ -473,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
-  if (PLANNED) pdl_wait();
+  ptx::grid_wait();
   const uint32_t tmem = bars->tmem;
   Jobs jobs{bars};
 
@@ -838,7 +836,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(256) combine_kernel(const Params p) {
   using E = ElemOps<T>;
   constexpr int PER = D / 32;
-  pdl_wait();
+  ptx::grid_wait();
   const int lane = threadIdx.x & 31;
   const int rows_per_item = 2 * p.tile_pos * p.group;
   const long long total = (long long)p.header->n_splits * p.kv_heads * p.rows_cap;
@@ -903,23 +901,6 @@ gdc_status encode(CUtensorMap* map, bool bf16, const void* base, int rank, const
          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return set_error(GDC_ERR_CUDA, "cuTensorMapEncodeTiled (packed attention) failed (%d)", int(r));
   return GDC_OK;
-}
-
-// Launch whose kernel may start while the kernel before it on the stream still runs; it waits for
-// that one's results itself (griddepcontrol.wait).
-template <typename... KArgs, typename... Args>
-cudaError_t launch_after(void (*kern)(KArgs...), int grid, int threads, size_t smem, cudaStream_t stream, Args... args) {
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(grid));
-  cfg.blockDim = dim3(unsigned(threads));
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
 template <typename T, int D>
@@ -989,17 +970,17 @@ gdc_status launch_typed(const PackedAttentionArgs& a, cudaStream_t stream, int* 
   }));
   if (ce != cudaSuccess) return set_error(GDC_ERR_CUDA, "packed attention smem attribute: %s", cudaGetErrorString(ce));
   if (!l.planned) {
-    packed_attention_kernel<T, D, false><<<unsigned(l.items_ub * a.kv_heads), kThreads, S::kSmemBytes, stream>>>(tq, tk, tv, p);
-    return check_launch("packed_attention_kernel");
+    GDC_CUDA_TRY(launch_overlapped(packed_attention_kernel<T, D, false>, unsigned(l.items_ub * a.kv_heads), kThreads, S::kSmemBytes, 1,
+                                   stream, tq, tk, tv, p));
+    return GDC_OK;
   }
-  plan_kernel<<<1, kPlanThreads, 0, stream>>>(p);
-  GDC_TRY(check_launch("plan_kernel"));
+  GDC_CUDA_TRY(launch_overlapped(plan_kernel, 1, kPlanThreads, 0, 1, stream, p));
   const int64_t jobs = int64_t(l.chunks_cap) * a.kv_heads;
-  GDC_CUDA_TRY(launch_after(packed_attention_kernel<T, D, true>, int(std::min<int64_t>(sms, jobs)), kThreads, S::kSmemBytes, stream, tq,
-                            tk, tv, p));
+  GDC_CUDA_TRY(launch_overlapped(packed_attention_kernel<T, D, true>, unsigned(std::min<int64_t>(sms, jobs)), kThreads, S::kSmemBytes, 1,
+                                 stream, tq, tk, tv, p));
   if (l.split) {
     const int64_t rows = l.items_ub * a.kv_heads * l.rows_cap;
-    GDC_CUDA_TRY(launch_after(combine_kernel<T, D>, int(std::min<int64_t>(4 * sms, (rows + 7) / 8)), 256, 0, stream, p));
+    GDC_CUDA_TRY(launch_overlapped(combine_kernel<T, D>, unsigned(std::min<int64_t>(4 * sms, (rows + 7) / 8)), 256, 0, 1, stream, p));
   }
   return GDC_OK;
 }

@@ -435,6 +435,17 @@ __host__ __device__ constexpr uint32_t idesc_f16_f32(uint32_t M, uint32_t N, uin
   return (1u << 4) | (b_mn_major << 16) | ((N >> 3) << 17) | ((M >> 4) << 24);
 }
 
+// ---------------------------------------------------------------- kernel overlap
+
+// Waits until the kernels before this one on its stream have completed and their writes are
+// visible (a kernel launched with programmatic stream serialisation may start before that).
+// Every thread that goes on to read or write global memory calls it first, and every CTA calls
+// it, so that a later kernel's wait for this one covers the earlier ones too.
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// Lets the next kernel of the stream start its set-up once every CTA has called this.
+__device__ __forceinline__ void grid_launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // ---------------------------------------------------------------- misc
 
 __device__ __forceinline__ float warp_sum(float v) {
