@@ -1,7 +1,8 @@
 // out = residual + act(a . w^T + bias) on tcgen05 tensor cores, any M, N and K.
 //
 // The product is computed transposed: the MMA's 128 rows are weight rows (output columns n) and
-// its N dimension is `bt` rows of a (m), bt a multiple of 16 up to 256 chosen per call. So
+// its N dimension is `bt` rows of a (m), chosen per call: a multiple of 16 up to 256, or one of 32 up
+// to 512 as two MMAs side by side. So
 //   * few rows of a cost a narrow MMA (bt = 16 for a single token) while the weights, which are
 //     then all the traffic, stream through the wide operand;
 //   * in the epilogue a thread owns one n (its bias is one register) and walks over m: a warp
@@ -10,8 +11,8 @@
 //
 // Two forms, one kernel:
 //   PAIR    two CTAs (cta_group::2) make a 256 (n) x bt (m) tile: each loads its 128 weight rows
-//           and half of the a rows, the leader issues the MMAs for both. Persistent, two
-//           accumulators in TMEM, so a tile's epilogue runs beside the next tile's products.
+//           and half of the a rows, the leader issues the MMAs for both. Persistent; up to bt = 256
+//           two accumulators in TMEM, so a tile's epilogue runs beside the next tile's products.
 //   single  a CTA makes a 128 x bt tile; where tiles are fewer than SMs, a cluster of 2, 4 or 8 CTAs
 //           splits K, and each sums its share of the columns from all of them, in rank order,
 //           through distributed shared memory.
@@ -54,7 +55,7 @@ struct LinearParams {
   void* out;
   long long ldr, ldo, m_cap;
   const int32_t* rows_dev;
-  int N, K, bt, split, stages, stage_bytes;
+  int N, K, bt, subs, split, stages, stage_bytes;  // subs: MMAs side by side in a tile
   int acc_cols, tmem_cols;  // TMEM columns between accumulators, and in all
   int* err;
 };
@@ -196,7 +197,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int kb0 = PAIR ? 0 : int((long long)kblocks * rank / p.split);
   const int kb1 = PAIR ? kblocks : int((long long)kblocks * (rank + 1) / p.split);
   const int a_rows = PAIR ? bt / 2 : bt;  // rows of a this CTA loads
-  const int a_atom = a_rows * 128;
+  const int sub_rows = a_rows / p.subs, a_atom = sub_rows * 128, sub_bytes = 2 * a_atom;  // [sub][atom][rows][64]
 
   if (warp == 0) {
     if (lane == 0) {
@@ -204,7 +205,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t phase = 0;
       long long issued = 0;
       bool ok = true;
-      const uint32_t tx = uint32_t(PAIR ? 2 : 1) * uint32_t(kWBytes + 2 * a_atom);
+      const uint32_t tx = uint32_t(PAIR ? 2 : 1) * uint32_t(kWBytes + p.subs * sub_bytes);
       for (long long t = first; t < tiles && ok; t += stride) {
         int nb, mb;
         tile_at(t, num_n, num_m, nb, mb);
@@ -212,19 +213,21 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!(ok = ptx::mbar_wait(&empty[stage], phase ^ 1u, p.err))) break;
           uint8_t* s_w = ring + stage * p.stage_bytes;
           uint8_t* s_a = s_w + kWBytes;
-          const int n0 = nb * kTileN + int(PAIR ? rank * 128 : 0), m0 = mb * bt + int(PAIR ? rank * a_rows : 0);
+          const int n0 = nb * kTileN + int(PAIR ? rank * 128 : 0), m0 = mb * bt + int(PAIR ? rank * sub_rows : 0);
           if (PAIR) {
             const uint32_t bar = ptx::mapa_shared(ptx::smem_u32(&full[stage]), 0);
             if (leader) ptx::mbar_arrive_expect_tx(&full[stage], tx);
             for (int u = 0; u < 2; ++u) {
               ptx::tma_load_2d_pair(s_w + u * 16384, &tm_w, kb * kBK + u * 64, n0, bar);
-              ptx::tma_load_2d_pair(s_a + u * a_atom, &tm_a, kb * kBK + u * 64, m0, bar);
+              for (int h = 0; h < p.subs; ++h)
+                ptx::tma_load_2d_pair(s_a + h * sub_bytes + u * a_atom, &tm_a, kb * kBK + u * 64, m0 + h * 2 * sub_rows, bar);
             }
           } else {
             ptx::mbar_arrive_expect_tx(&full[stage], tx);
             for (int u = 0; u < 2; ++u) {
               ptx::tma_load_2d(s_w + u * 16384, &tm_w, kb * kBK + u * 64, n0, &full[stage]);
-              ptx::tma_load_2d(s_a + u * a_atom, &tm_a, kb * kBK + u * 64, m0, &full[stage]);
+              for (int h = 0; h < p.subs; ++h)
+                ptx::tma_load_2d(s_a + h * sub_bytes + u * a_atom, &tm_a, kb * kBK + u * 64, m0 + h * sub_rows, &full[stage]);
             }
           }
           ++issued;
@@ -247,7 +250,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == 1) {
     if (lane == 0 && leader) {
       const uint32_t idesc =
-          ptx::idesc_f16_f32(PAIR ? 256 : 128, uint32_t(bt)) | (E::kMmaFormat << 7) | (E::kMmaFormat << 10);
+          ptx::idesc_f16_f32(PAIR ? 256 : 128, uint32_t(bt / p.subs)) | (E::kMmaFormat << 7) | (E::kMmaFormat << 10);
       int stage = 0, local = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -260,14 +263,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!(ok = ptx::mbar_wait(&full[stage], phase, p.err))) break;
           ptx::tc_fence_after();
           const uint32_t w_addr = ptx::smem_u32(ring + stage * p.stage_bytes), a_addr = w_addr + kWBytes;
+          for (int h = 0; h < p.subs; ++h) {
+            const uint32_t dh = d + uint32_t(h * (bt / 2));
 #pragma unroll
-          for (int k = 0; k < kBK / 16; ++k) {
-            const uint64_t dw = ptx::desc_kmajor_sw128(w_addr + (k >> 2) * 16384 + (k & 3) * 32);
-            const uint64_t da = ptx::desc_kmajor_sw128(a_addr + (k >> 2) * a_atom + (k & 3) * 32);
-            if (PAIR)
-              ptx::umma_f16_ss_pair(d, dw, da, idesc, (kb != kb0) | (k != 0));
-            else
-              ptx::umma_f16_ss(d, dw, da, idesc, (kb != kb0) | (k != 0));
+            for (int k = 0; k < kBK / 16; ++k) {
+              const uint64_t dw = ptx::desc_kmajor_sw128(w_addr + (k >> 2) * 16384 + (k & 3) * 32);
+              const uint64_t da = ptx::desc_kmajor_sw128(a_addr + h * sub_bytes + (k >> 2) * a_atom + (k & 3) * 32);
+              if (PAIR)
+                ptx::umma_f16_ss_pair(dh, dw, da, idesc, (kb != kb0) | (k != 0));
+              else
+                ptx::umma_f16_ss(dh, dw, da, idesc, (kb != kb0) | (k != 0));
+            }
           }
           if (PAIR)
             ptx::umma_commit_pair_mc(&empty[stage], 0x3);
@@ -328,30 +334,34 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         break;  // one tile a cluster; finished below
       }
+      const bool has_res = col.res != nullptr && live;
+      const int count = (chunks - part + 3) / 4;  // chunks part, part + 4, ...
       uint16_t r[3][16];
-      if (col.res != nullptr && live) {
+      if (has_res) {
 #pragma unroll
         for (int u = 0; u < 3; ++u)
-          if (part + 4 * u < chunks) col.fetch(m_tile + (part + 4 * u) * 16, r[u]);
+          if (u < count) col.fetch(m_tile + (part + 4 * u) * 16, r[u]);
       }
       if (!__all_sync(0xffffffffu, ptx::mbar_wait(&tfull[acc], (local >> 1) & 1, p.err))) break;
       ptx::tc_fence_after();
+      for (int i = 0; i < count; i += 3) {
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int c = part + 4 * u;
-        if (c < chunks) {
-          uint32_t z[16];
-          ptx::tmem_ld_32x32b_x16(t_row + c * 16, z);
-          ptx::tmem_wait_ld();
-          if (live) col.store(m_tile + c * 16, z, r[u % 3]);
-          if (u == 0 && col.res != nullptr && live && part + 12 < chunks) col.fetch(m_tile + (part + 12) * 16, r[0]);
+        for (int u = 0; u < 3; ++u) {
+          if (i + u < count) {
+            const int c = part + 4 * (i + u);
+            uint32_t z[16];
+            ptx::tmem_ld_32x32b_x16(t_row + c * 16, z);
+            ptx::tmem_wait_ld();
+            if (live) col.store(m_tile + c * 16, z, r[u]);
+            if (has_res && i + u + 3 < count) col.fetch(m_tile + (c + 12) * 16, r[u]);
+          }
         }
       }
       ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) {
         if (PAIR)
-          ptx::mbar_arrive_cluster(ptx::mapa_shared(ptx::smem_u32(&tempty[acc]), 0));
+          ptx::mbar_arrive_cluster_relaxed(ptx::mapa_shared(ptx::smem_u32(&tempty[acc]), 0));
         else
           ptx::mbar_arrive(&tempty[acc]);
       }
@@ -412,35 +422,45 @@ struct Config {
   int bt, split;
 };
 
-// The form of a call: the estimated time (in tensor-core cycles) of every form is its rounds over
-// the SMs times a tile's time; the least wins.
-Config choose(int64_t M, int N, int K, int sms) {
+// What a device can run at once: SMs, and clusters of 2, 4 and 8 CTAs of the single form.
+struct DeviceLimits {
+  int sms = 148, clusters[4] = {148, 74, 36, 16};
+};
+
+// The form of a call: each form's estimated time in microseconds; the least wins. Measured on a
+// B200: operand tiles arrive at 95 bytes a nanosecond and SM when all SMs load, 130 when half of
+// them do (this, not the tensor cores, bounds every tile below 256 x 256); an epilogue takes 11 ns
+// a column, 9 more for a residual or a GELU; joining split K about 1.2 us.
+Config choose(int64_t M, int N, int K, bool residual, int act, const DeviceLimits& dev) {
   Config best{false, 16, 1};
-  double best_cost = 1e300;
-  const double kblocks = double((K + kBK - 1) / kBK);
+  double best_time = 1e300;
+  const int64_t kblocks = (K + kBK - 1) / kBK;
   auto consider = [&](const Config& c) {
     const int64_t tile_n = c.pair ? 256 : 128;
     const int64_t tiles = ((N + tile_n - 1) / tile_n) * ((M + c.bt - 1) / c.bt);
-    const int64_t ctas = tiles * (c.pair ? 2 : c.split);
-    if (c.split > 1 && ctas > sms) return;
-    const double rounds = double(c.pair ? (tiles + sms / 2 - 1) / (sms / 2) : (ctas + sms - 1) / sms);
-    // a K block: the MMA's own cycles (8 of K = 16, bt / 2 cycles each), or the shared-memory traffic of its
-    // operands where that is more
+    const int64_t at_once = c.pair ? dev.clusters[1] : (c.split == 1 ? dev.sms : dev.clusters[c.split == 2 ? 1 : c.split == 4 ? 2 : 3]);
+    if (c.split > 1 && tiles > at_once) return;
+    const int64_t rounds = (tiles + at_once - 1) / at_once;
+    if (c.bt > 256 && rounds > 1) return;  // one accumulator only
+    const double ctas = double(std::min(tiles, at_once)) * (c.pair ? 2 : c.split);
+    const double rate = ctas > dev.sms / 2 ? 95e3 : 130e3;
     const double a_rows = c.pair ? c.bt / 2 : c.bt;
-    const double block = std::max(4.0 * c.bt, (128 + a_rows) * kBK * 2 * 2 / 128.0);
-    const double cost = rounds * (kblocks / c.split * block + 300) + (c.split > 1 ? 600 : 0) + 8.0 * c.bt;
-    if (cost < best_cost * 0.999) {
-      best_cost = cost;
+    const double block = std::max((128 + a_rows) * kBK * 2 / rate, 4.0 * c.bt / 1850.0);
+    const double main = double((kblocks + c.split - 1) / c.split) * block;
+    const double epilogue = c.bt * (0.011 + (residual ? 0.009 : 0) + (act == kActGelu ? 0.009 : 0)) / c.split + (c.split > 1 ? 1.2 : 0);
+    const double time = main + double(rounds - 1) * std::max(main, epilogue) + epilogue;
+    if (time < best_time * 0.999) {
+      best_time = time;
       best = c;
     }
   };
-  const int bt_max = int(std::min<int64_t>(256, (M + 15) / 16 * 16));
-  for (int bt = bt_max; bt >= 16; bt -= 16) {
-    if (M > 128 && bt >= 32) consider({true, bt, 1});
+  const int64_t bt_max = std::min<int64_t>(512, (M + 15) / 16 * 16);
+  for (int bt = 16; bt <= bt_max || bt == 16; bt += bt < 256 ? 16 : 32) {
+    if (M > 64 && bt >= 32) consider({true, bt, 1});
     consider({false, bt, 1});
     if (bt <= kMaxSplitBt)
       for (int s = 2; s <= 8; s *= 2)
-        if (s <= int(kblocks)) consider({false, bt, s});
+        if (s <= kblocks) consider({false, bt, s});
   }
   return best;
 }
@@ -458,18 +478,49 @@ gdc_status launch_form(const CUtensorMap& tw, const CUtensorMap& ta, const Linea
   return GDC_OK;
 }
 
+// Limits of a device, asked once: how many clusters fit depends on how its SMs are grouped.
+gdc_status device_limits(int dev, DeviceLimits* out) {
+  static PerDeviceOnce once;
+  static DeviceLimits limits[64];
+  auto kern = linear_residual_kernel<__half, false, kActNone>;
+  const cudaError_t ce = cudaError_t(per_device_once(once, dev, [&] {
+    DeviceLimits& l = limits[dev];
+    l.sms = l.clusters[0] = device_sm_count(dev);
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+    for (int i = 1; i < 4 && e == cudaSuccess; ++i) {
+      cudaLaunchAttribute attr{};
+      attr.id = cudaLaunchAttributeClusterDimension;
+      attr.val.clusterDim.x = 1u << i;
+      attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+      cudaLaunchConfig_t cfg{};
+      cfg.gridDim = dim3(unsigned(l.sms) >> i << i);
+      cfg.blockDim = dim3(kThreads);
+      cfg.dynamicSmemBytes = kMaxSmem;
+      cfg.attrs = &attr;
+      cfg.numAttrs = 1;
+      e = cudaOccupancyMaxActiveClusters(&l.clusters[i], kern, &cfg);
+    }
+    return e;
+  }));
+  if (ce != cudaSuccess) return set_error(GDC_ERR_CUDA, "linear residual cluster limits: %s", cudaGetErrorString(ce));
+  *out = limits[dev];
+  return GDC_OK;
+}
+
 template <typename T>
 gdc_status launch_typed(const LinearResidualArgs& a, cudaStream_t stream, int* err) {
   constexpr bool bf16 = ElemOps<T>::kMmaFormat == 1;
   int dev = 0;
   GDC_CUDA_TRY(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64) return set_error(GDC_ERR_CUDA, "device ordinal out of range");
-  const int sms = device_sm_count(dev);
-  const Config c = choose(a.M, a.N, a.K, sms);
-  const int a_rows = c.pair ? c.bt / 2 : c.bt;
+  DeviceLimits lim;
+  GDC_TRY(device_limits(dev, &lim));
+  const int sms = lim.sms;
+  const Config c = choose(a.M, a.N, a.K, a.residual != nullptr, a.act, lim);
+  const int a_rows = c.pair ? c.bt / 2 : c.bt, subs = c.bt > 256 ? 2 : 1;
   CUtensorMap tw, ta;
   GDC_TRY(encode(&tw, bf16, a.w, uint64_t(a.N), uint64_t(a.K), uint64_t(a.ldw), 128));
-  GDC_TRY(encode(&ta, bf16, a.a, uint64_t(a.M), uint64_t(a.K), uint64_t(a.lda), uint32_t(a_rows)));
+  GDC_TRY(encode(&ta, bf16, a.a, uint64_t(a.M), uint64_t(a.K), uint64_t(a.lda), uint32_t(a_rows / subs)));
   LinearParams p{};
   p.bias = a.bias;
   p.residual = a.residual;
@@ -481,21 +532,24 @@ gdc_status launch_typed(const LinearResidualArgs& a, cudaStream_t stream, int* e
   p.N = a.N;
   p.K = a.K;
   p.bt = c.bt;
+  p.subs = subs;
   p.split = c.split;
   p.stage_bytes = kWBytes + a_rows * kBK * 2;
-  // A call of one round keeps to a small ring and little TMEM, so that the next kernel's set-up can
-  // run beside it; more rounds use the SM's whole shared memory.
   const int64_t tile_n = c.pair ? 256 : 128;
   const int64_t tiles = ((a.N + tile_n - 1) / tile_n) * ((a.M + c.bt - 1) / c.bt);
-  const bool small = tiles * (c.pair ? 2 : c.split) <= sms;
-  p.stages = std::min(kMaxStages, (small ? kSmallRing : kRingBytes) / p.stage_bytes);
-  if (p.stages < 2) p.stages = kRingBytes / p.stage_bytes;
+  const int64_t at_once = c.pair ? lim.clusters[1] : (c.split == 1 ? sms : tiles);
+  const int64_t blocks = ((a.K + kBK - 1) / kBK + c.split - 1) / c.split;  // K blocks of a CTA's tile
+  // A ring holds what it can use. One that stays small leaves room for the next kernel's set-up on
+  // the SM; a tile of more K blocks than fit there uses the SM's whole shared memory.
+  const bool one = tiles <= at_once;
+  const int deep = std::min(kMaxStages, kRingBytes / p.stage_bytes), shallow = std::min(kMaxStages, kSmallRing / p.stage_bytes);
+  p.stages = one && blocks <= shallow ? int(std::max<int64_t>(1, blocks)) : deep;
   p.acc_cols = (c.bt + 31) / 32 * 32;
   p.tmem_cols = 32;
-  while (p.tmem_cols < (small ? 1 : 2) * p.acc_cols) p.tmem_cols *= 2;
+  while (p.tmem_cols < (one ? 1 : 2) * p.acc_cols) p.tmem_cols *= 2;
   p.err = err;
   const int cluster = c.pair ? 2 : c.split;
-  const int grid = c.pair ? 2 * int(std::min<int64_t>(tiles, sms / 2))
+  const int grid = c.pair ? 2 * int(std::min<int64_t>(tiles, at_once))
                           : (c.split > 1 ? int(tiles * c.split) : int(std::min<int64_t>(tiles, sms)));
   switch (a.act * 2 + c.pair) {
     case 2 * kActNone: return launch_form<T, false, kActNone>(tw, ta, p, grid, cluster, stream, dev);
