@@ -44,11 +44,12 @@ constexpr int kEpiWarps = 16;    // four a TMEM lane quarter, each every fourth 
 constexpr int kThreads = 64 + 32 * kEpiWarps;
 constexpr int kMaxStages = 6;
 constexpr int kWBytes = 128 * kBK * 2;
-constexpr int kRingBytes = 192 * 1024;
+constexpr int kRingBytes = 225 * 1024, kSplitRing = 192 * 1024;  // (split K keeps partial sums beside the ring)
 constexpr int kSmallRing = 108 * 1024;  // leaves room for a second CTA's set-up on the SM
 constexpr int kMaxSplitBt = 64;  // split K: columns x 128 lanes x 4 bytes of partial sums, 32 KB
 constexpr int kCtrlBytes = 256;
-constexpr int kMaxSmem = kRingBytes + kMaxSplitBt * 512 + kCtrlBytes + 1024;
+constexpr int kMaxSmem = kRingBytes + kCtrlBytes + 1024;
+static_assert(kSplitRing + kMaxSplitBt * 512 <= kRingBytes && kMaxSmem <= 232448, "shared memory of a CTA");
 
 struct LinearParams {
   const void *bias, *residual;
@@ -137,7 +138,7 @@ template <typename T, bool PAIR, int ACT>
 __global__ void __launch_bounds__(kThreads, 1)
     linear_residual_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a, const LinearParams p) {
   using E = ElemOps<T>;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = ptx::warp_index(), lane = threadIdx.x & 31;
   ptx::grid_launch_next();
   if (threadIdx.x == 0) {
     ptx::prefetch_tensor_map(&tm_w);
@@ -248,7 +249,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && leader) {
+    if (leader) {
       const uint32_t idesc =
           ptx::idesc_f16_f32(PAIR ? 256 : 128, uint32_t(bt / p.subs)) | (E::kMmaFormat << 7) | (E::kMmaFormat << 10);
       int stage = 0, local = 0;
@@ -256,11 +257,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       for (long long t = first; t < tiles && ok; t += stride, ++local) {
         const int acc = local & 1;
-        if (!(ok = ptx::mbar_wait(&tempty[acc], ((local >> 1) & 1) ^ 1, p.err))) break;
+        if (!(ok = __all_sync(0xffffffffu, ptx::mbar_wait(&tempty[acc], ((local >> 1) & 1) ^ 1, p.err)))) break;
         ptx::tc_fence_after();
         const uint32_t d = tmem + uint32_t(acc * p.acc_cols);
         for (int kb = kb0; kb < kb1; ++kb) {
-          if (!(ok = ptx::mbar_wait(&full[stage], phase, p.err))) break;
+          if (!(ok = __all_sync(0xffffffffu, ptx::mbar_wait(&full[stage], phase, p.err)))) break;
           ptx::tc_fence_after();
           const uint32_t w_addr = ptx::smem_u32(ring + stage * p.stage_bytes), a_addr = w_addr + kWBytes;
           for (int h = 0; h < p.subs; ++h) {
@@ -270,15 +271,15 @@ __global__ void __launch_bounds__(kThreads, 1)
               const uint64_t dw = ptx::desc_kmajor_sw128(w_addr + (k >> 2) * 16384 + (k & 3) * 32);
               const uint64_t da = ptx::desc_kmajor_sw128(a_addr + h * sub_bytes + (k >> 2) * a_atom + (k & 3) * 32);
               if (PAIR)
-                ptx::umma_f16_ss_pair(dh, dw, da, idesc, (kb != kb0) | (k != 0));
+                ptx::umma_f16_ss_pair_warp(dh, dw, da, idesc, (kb != kb0) | (k != 0));
               else
-                ptx::umma_f16_ss(dh, dw, da, idesc, (kb != kb0) | (k != 0));
+                ptx::umma_f16_ss_warp(dh, dw, da, idesc, (kb != kb0) | (k != 0));
             }
           }
           if (PAIR)
-            ptx::umma_commit_pair_mc(&empty[stage], 0x3);
+            ptx::umma_commit_pair_mc_warp(&empty[stage], 0x3);
           else
-            ptx::umma_commit(&empty[stage]);
+            ptx::umma_commit_warp(&empty[stage]);
           if (++stage == p.stages) {
             stage = 0;
             phase ^= 1u;
@@ -286,15 +287,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (!ok) break;
         if (PAIR)
-          ptx::umma_commit_pair_mc(&tfull[acc], 0x3);
+          ptx::umma_commit_pair_mc_warp(&tfull[acc], 0x3);
         else
-          ptx::umma_commit(&tfull[acc]);
+          ptx::umma_commit_warp(&tfull[acc]);
       }
       // every issued MMA is done before TMEM is released
       if (PAIR)
-        ptx::umma_commit_pair(ptx::mapa_shared(ptx::smem_u32(drain), 0));
+        ptx::umma_commit_pair_mc_warp(drain, 0x1);
       else
-        ptx::umma_commit(drain);
+        ptx::umma_commit_warp(drain);
       const unsigned long long t0 = ptx::globaltimer();
       while (!ptx::mbar_try_wait(drain, 0) && ptx::globaltimer() - t0 < ptx::kTimeoutNs) {
       }
@@ -542,7 +543,7 @@ gdc_status launch_typed(const LinearResidualArgs& a, cudaStream_t stream, int* e
   // A ring holds what it can use. One that stays small leaves room for the next kernel's set-up on
   // the SM; a tile of more K blocks than fit there uses the SM's whole shared memory.
   const bool one = tiles <= at_once;
-  const int deep = std::min(kMaxStages, kRingBytes / p.stage_bytes), shallow = std::min(kMaxStages, kSmallRing / p.stage_bytes);
+  const int deep = std::min(kMaxStages, (c.split > 1 ? kSplitRing : kRingBytes) / p.stage_bytes), shallow = std::min(kMaxStages, kSmallRing / p.stage_bytes);
   p.stages = one && blocks <= shallow ? int(std::max<int64_t>(1, blocks)) : deep;
   p.acc_cols = (c.bt + 31) / 32 * 32;
   p.tmem_cols = 32;
