@@ -437,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* s_q = smem + S::kOffQ;
   uint8_t* s_ring = smem + S::kOffRing;
   Bars* bars = reinterpret_cast<Bars*>(smem + S::kOffBar);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = ptx::warp_index(), lane = threadIdx.x & 31;
   int* err = p.err;
 
   ptx::grid_launch_next();
@@ -568,11 +568,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           const uint32_t off = uint32_t(k >> 2) * 16384 + (k & 3) * 32;
-          ptx::umma_f16_ss(tmem + t * 128, ptx::desc_kmajor_sw128(q_addr + off), ptx::desc_kmajor_sw128(k_addr + off), idesc_s,
-                           k != 0);
+          ptx::umma_f16_ss_warp(tmem + t * 128, ptx::desc_kmajor_sw128(q_addr + off), ptx::desc_kmajor_sw128(k_addr + off), idesc_s,
+                                k != 0);
         }
-        ptx::umma_commit(&bars->s_full[t]);
-        if (j + 1 == cnt[t]) ptx::umma_commit(&bars->q_empty[t]);
+        ptx::umma_commit_warp(&bars->s_full[t]);
+        if (j + 1 == cnt[t]) ptx::umma_commit_warp(&bars->q_empty[t]);
       };
       // S_t(0)
       ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->full[stage], phase, err));
@@ -581,10 +581,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (ok && cnt[t] > 0) {
           ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->q_full[t], items_of[t] & 1, err));
           ptx::tc_fence_after();
-          if (ok && lane == 0) scores(t, 0, ptx::smem_u32(s_ring + stage * S::kTileBytes));
+          if (ok) scores(t, 0, ptx::smem_u32(s_ring + stage * S::kTileBytes));
         }
       if (!ok) break;
-      if (lane == 0) ptx::umma_commit(&bars->empty[stage]);
+      ptx::umma_commit_warp(&bars->empty[stage]);
       advance();
       for (int j = 0; j < n && ok; ++j) {
         const int v_stage = stage;
@@ -614,10 +614,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (ok && j == 0) ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->o_free[t], (items_of[t] & 1) ^ 1, err));
           if (!ok) continue;
           ptx::tc_fence_after();
-          if (lane == 0) {
+          {
 #pragma unroll
             for (int k = 0; k < kKeys / 16; ++k)
-              ptx::umma_f16_ts(tmem + 256 + t * D, tmem + t * 128 + k * 8, desc_v(v_addr + k * 2048), idesc_o, (j | k) != 0);
+              ptx::umma_f16_ts_warp(tmem + 256 + t * D, tmem + t * 128 + k * 8, desc_v(v_addr + k * 2048), idesc_o, (j | k) != 0);
           }
           if (j + 1 < cnt[t]) {
             if (!k_ready) {
@@ -626,15 +626,15 @@ __global__ void __launch_bounds__(kThreads, 1)
               ptx::tc_fence_after();
               k_ready = true;
             }
-            if (lane == 0) scores(t, j + 1, ptx::smem_u32(s_ring + stage * S::kTileBytes));
+            scores(t, j + 1, ptx::smem_u32(s_ring + stage * S::kTileBytes));
           } else {
-            if (lane == 0) ptx::umma_commit(&bars->o_full[t]);
+            ptx::umma_commit_warp(&bars->o_full[t]);
           }
         }
         if (!ok) break;
-        if (lane == 0) ptx::umma_commit(&bars->empty[v_stage]);
+        ptx::umma_commit_warp(&bars->empty[v_stage]);
         if (more) {
-          if (lane == 0) ptx::umma_commit(&bars->empty[stage]);
+          ptx::umma_commit_warp(&bars->empty[stage]);
           advance();
         }
       }
@@ -642,9 +642,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int t = 0; t < 2; ++t)
         if (cnt[t] > 0) ++items_of[t];
     }
+    // every issued MMA is done before TMEM is released
+    ptx::umma_commit_warp(&bars->drain);
     if (lane == 0) {
-      // every issued MMA is done before TMEM is released
-      ptx::umma_commit(&bars->drain);
       const unsigned long long t0 = ptx::globaltimer();
       while (!ptx::mbar_try_wait(&bars->drain, 0) && ptx::globaltimer() - t0 < ptx::kTimeoutNs) {
       }
