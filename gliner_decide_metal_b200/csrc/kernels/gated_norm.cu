@@ -7,10 +7,10 @@
 // row with a large mean loses nothing.
 //
 // What bounds it is bytes in flight: the sums are a chain of up to four reductions a row. So the
-// grid is persistent and every thread has its values of the next two rows on their way to its own
+// grid is persistent and every thread has its values of the next row on their way to its own
 // slots of shared memory (cp.async; no other thread reads them, so nothing is synchronised) while
-// it works on this one, and a row belongs to as few threads as hold it in registers: one warp up to 1024
-// columns (reductions without a barrier, four rows a block), one block of 128 to 512 threads above.
+// it works on this one, and a row belongs to few threads: one warp up to 512
+// columns (reductions without a barrier, four rows a block), one block of 64 to 512 threads above.
 // Weights and gate rows are read again for every row, from L1. Rows at odd 2-byte addresses are read
 // value by value when their turn comes.
 #include <algorithm>
@@ -131,7 +131,7 @@ __device__ __forceinline__ float row_sum(float v, float* red, int& turn) {
   return s;
 }
 
-// v <- N(v); values at or past `cols` are zero and stay out of the sums.
+// v <- N(v); values at or past `cols` stay out of the sums.
 template <typename T, int V, int N, int TPR>
 __device__ __forceinline__ void normalise(float (&v)[N], int kind, const T* w, const T* b, int first, int step, int cols, float inv_cols,
                                           float eps, float* red, int& turn) {
@@ -139,19 +139,23 @@ __device__ __forceinline__ void normalise(float (&v)[N], int kind, const T* w, c
   if (kind == 1) {
     float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) s += v[i];
+    for (int c = 0; c < N / V; ++c)
+      if (first + c * step < cols) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) s += v[c * V + j];
+      }
     mean = row_sum<TPR>(s, red, turn) * inv_cols;
   }
   float q = 0.f;
 #pragma unroll
-  for (int c = 0; c < N / V; ++c) {
-    const bool in = first + c * step < cols;
+  for (int c = 0; c < N / V; ++c)
+    if (first + c * step < cols) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float d = v[c * V + j] - mean;
-      q += in ? d * d : 0.f;
+      for (int j = 0; j < V; ++j) {
+        const float d = v[c * V + j] - mean;
+        q = fmaf(d, d, q);
+      }
     }
-  }
   const float inv = rsqrtf(row_sum<TPR>(q, red, turn) * inv_cols + eps);
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = (v[i] - mean) * inv;
@@ -177,7 +181,7 @@ __device__ __forceinline__ void normalise(float (&v)[N], int kind, const T* w, c
   }
 }
 
-constexpr int kStages = 3;  // rows of a thread in shared memory: the current one and the next two
+constexpr int kStages = 2;  // rows of a thread in shared memory: the current one and the next (a third costs the weights their L1)
 
 template <int V, int N, int TPR>
 struct NormShape {
@@ -185,7 +189,7 @@ struct NormShape {
   static constexpr bool kAsync = V > 1;
   static constexpr int kRowBytes = kThreads * N * 2;  // one tensor of the block's rows
   static constexpr int kSmemBytes = kAsync ? kStages * 2 * kRowBytes : 0;
-  static constexpr int kBlocks = N == 32 ? (TPR == 32 ? 4 : 1) : 1024 / kThreads;  // resident on an SM
+  static constexpr int kBlocks = N == 32 ? (TPR <= 128 ? 4 : TPR == 256 ? 2 : 1) : 1024 / kThreads;  // resident on an SM
 };
 
 template <typename T, int V, int N, int TPR>
@@ -262,11 +266,7 @@ __global__ void __launch_bounds__(NormShape<V, N, TPR>::kThreads, NormShape<V, N
         }
       }
 #pragma unroll
-      for (int c = 0; c < N / V; ++c) {
-        const bool in = first + c * step < cols;
-#pragma unroll
-        for (int j = 0; j < V; ++j) xv[c * V + j] = in ? fmaf(p.scale, z[c * V + j], xv[c * V + j]) : 0.f;
-      }
+      for (int i = 0; i < N; ++i) xv[i] = fmaf(p.scale, z[i], xv[i]);
     }
     if (p.x_out != nullptr) store<T, V, N>(static_cast<T*>(p.x_out) + row * p.ldxo, xv, first, step, cols);
     if (p.pre != 0) {
@@ -300,12 +300,15 @@ gdc_status launch_variant(const NormParams& p, cudaStream_t stream) {
 
 template <typename T, int V>
 gdc_status launch_width(const NormParams& p, cudaStream_t stream) {
+  // Values a thread and threads a row, measured: 16 x 64 against 32 x 32 at 1024 columns (16384 rows:
+  // 25.4 against 26.1 us; one row: 3.2 against 3.7; single values 8 x 128: 42 against 55), 32 x 128
+  // against 16 x 256 at 4096 (two LayerNorms over 16384 rows: 108 against 118 us).
   const int c = p.cols;
   if (c <= 256) return launch_variant<T, V, 8, 32>(p, stream);
   if (c <= 512) return launch_variant<T, V, 16, 32>(p, stream);
-  if (c <= 1024) return launch_variant<T, V, 32, 32>(p, stream);
+  if (c <= 1024) return V == 1 ? launch_variant<T, V, 8, 128>(p, stream) : launch_variant<T, V, 16, 64>(p, stream);
   if (c <= 2048) return launch_variant<T, V, 16, 128>(p, stream);
-  if (c <= 4096) return launch_variant<T, V, 16, 256>(p, stream);
+  if (c <= 4096) return launch_variant<T, V, 32, 128>(p, stream);
   if (c <= 8192) return launch_variant<T, V, 16, 512>(p, stream);
   return launch_variant<T, V, 32, 512>(p, stream);
 }
