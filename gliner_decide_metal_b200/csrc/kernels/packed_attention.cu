@@ -329,13 +329,15 @@ struct Shape {
   static constexpr int kOffQ = 0;
   static constexpr int kOffRing = 2 * kTileBytes;
   static constexpr int kOffBar = kOffRing + kStages * kTileBytes;
-  static constexpr int kSmemBytes = kOffBar + 512 + 1024;
+  static constexpr int kOffMl = kOffBar + 512;  // tile 1's references and sums of a shared item
+  static constexpr int kSmemBytes = kOffMl + 128 * 8 + 1024;
+  static_assert(kSmemBytes <= 232448, "shared memory of a CTA");
 };
 
 struct Bars {
   uint64_t full[10], empty[10];
   uint64_t q_full[2], q_empty[2], s_full[2], p_ready[2], o_full[2], o_free[2], drain;
-  uint64_t job_full[2], job_empty[2];
+  uint64_t job_full[2], job_empty[2], ml_ready;
   uint32_t tmem, pad;
   Job job[2];
 };
@@ -359,6 +361,14 @@ __device__ __forceinline__ int tile_count(const Params& p, const Item& it, int t
   const int last = min(first + p.tile_pos, it.lq) - 1;
   const int need = (seen_keys(last, it.lq, it.lk, p.causal) + kKeys - 1) / kKeys;
   return max(0, min(it.t1, need) - it.t0);
+}
+
+// An item whose rows fill one query tile at most and that has several key tiles (tokens taken one at a
+// time): both row groups work on that tile, group 0 on the even key tiles and group 1 on the odd ones,
+// each with its own reference, sum and O; group 0 joins them at the end. One group alone takes
+// about 1.9 us a 64 KB key and value tile, twice what memory needs for it.
+__device__ __forceinline__ bool shared_item(const Params& p, const Item& it) {
+  return it.pos + p.tile_pos >= it.lq && tile_count(p, it, 0) > 1;
 }
 
 // The CTA's next job, by its producer (one lane): planned ones from the list, every other round
@@ -461,6 +471,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       ptx::mbar_init(&bars->job_full[i], 1);
       ptx::mbar_init(&bars->job_empty[i], 9);  // the MMA warp and the eight row warps
     }
+    ptx::mbar_init(&bars->ml_ready, 4);
     ptx::mbar_init(&bars->drain, 1);
     ptx::fence_barrier_init();
   }
@@ -523,9 +534,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (n0 > 0) load_q(0);
         load_kv(&tm_k, 0);
         if (n1 > 0) load_q(1);
+        const int ahead = shared_item(p, it) ? 2 : 1;  // key tiles before the first value tile
+        if (ahead == 2) load_kv(&tm_k, 1);
         for (int j = 0; j < n && ok; ++j) {
           load_kv(&tm_v, j);
-          if (j + 1 < n) load_kv(&tm_k, j + 1);
+          if (j + ahead < n) load_kv(&tm_k, j + ahead);
         }
       }
       // the loads in flight land before the CTA can exit (bounded)
@@ -548,6 +561,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int stage = 0;
     uint32_t phase = 0;
     uint32_t items_of[2] = {0, 0}, p_uses[2] = {0, 0};
+    uint32_t q1_skipped = 0;  // shared items: group 1 took part without a query tile of its own
     bool ok = true;
     while (ok) {
       const Job* job = jobs.next(err);
@@ -555,6 +569,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int cnt[2] = {tile_count(p, job->it, 0), tile_count(p, job->it, 1)};
       const int n = max(cnt[0], cnt[1]);
       const int keys_left = job->it.lk - job->it.t0 * kKeys;
+      const bool shared = shared_item(p, job->it);
       jobs.done();
       if (n == 0) continue;
       auto advance = [&] {
@@ -563,8 +578,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           phase ^= 1;
         }
       };
-      auto scores = [&](int t, int j, uint32_t k_addr) {
-        const uint32_t q_addr = ptx::smem_u32(s_q + t * S::kTileBytes);
+      // S_t = Q_tq K^T
+      auto products = [&](int t, int tq, uint32_t k_addr) {
+        const uint32_t q_addr = ptx::smem_u32(s_q + tq * S::kTileBytes);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           const uint32_t off = uint32_t(k >> 2) * 16384 + (k & 3) * 32;
@@ -572,6 +588,74 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 k != 0);
         }
         ptx::umma_commit_warp(&bars->s_full[t]);
+      };
+      auto wait_tile = [&] {
+        const bool got = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->full[stage], phase, err));
+        ptx::tc_fence_after();
+        return got;
+      };
+      // value rows behind the sequence's last key (valid ones before them): zero, whatever the buffer holds there
+      auto zero_tail = [&](uint8_t* v_tile, int valid) {
+        if (valid >= kKeys) return;
+        for (int i = lane; i < (kKeys - valid) * 8; i += 32)
+#pragma unroll
+          for (int a = 0; a < S::kAtoms; ++a)
+            *reinterpret_cast<uint4*>(v_tile + a * 16384 + valid * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+      };
+      // O_t (+)= P_t V
+      auto values = [&](int t, uint32_t v_addr, bool first) {
+#pragma unroll
+        for (int k = 0; k < kKeys / 16; ++k)
+          ptx::umma_f16_ts_warp(tmem + 256 + t * D, tmem + t * 128 + k * 8, desc_v(v_addr + k * 2048), idesc_o, !first | (k != 0));
+      };
+      // the weights of P_t, and before its first product of an item, O_t's columns
+      auto weights_ready = [&](int t, bool first) {
+        bool got = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->p_ready[t], p_uses[t] & 1, err));
+        ++p_uses[t];
+        if (got && first) got = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->o_free[t], (items_of[t] & 1) ^ 1, err));
+        ptx::tc_fence_after();
+        return got;
+      };
+      if (shared) {
+        // tiles in the order K0 K1 V0 K2 V1 K3 ..., group j % 2 takes tile j
+        ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->q_full[0], items_of[0] & 1, err));
+        auto next_scores = [&](int t) {
+          ok = wait_tile();
+          if (!ok) return;
+          products(t, 0, ptx::smem_u32(s_ring + stage * S::kTileBytes));
+          ptx::umma_commit_warp(&bars->empty[stage]);
+          advance();
+        };
+        if (ok) next_scores(0);
+        if (ok) next_scores(1);
+        if (ok && n == 2) ptx::umma_commit_warp(&bars->q_empty[0]);
+        for (int j = 0; j < n && ok; j += 2) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (!ok || j + t >= n) continue;
+            if (!(ok = wait_tile())) continue;
+            zero_tail(s_ring + stage * S::kTileBytes, keys_left - (j + t) * kKeys);
+            if (!(ok = weights_ready(t, j == 0))) continue;
+            values(t, ptx::smem_u32(s_ring + stage * S::kTileBytes), j == 0);
+            ptx::umma_commit_warp(&bars->empty[stage]);
+            advance();
+            if (j + t + 2 < n) {
+              next_scores(t);
+              if (ok && j + t + 3 == n) ptx::umma_commit_warp(&bars->q_empty[0]);
+            } else {
+              ptx::umma_commit_warp(&bars->o_full[t]);
+            }
+          }
+        }
+        ++items_of[0];
+        ++items_of[1];
+        ++q1_skipped;
+        continue;
+      }
+      auto scores = [&](int t, int j, uint32_t k_addr) {
+        products(t, t, k_addr);
         if (j + 1 == cnt[t]) ptx::umma_commit_warp(&bars->q_empty[t]);
       };
       // S_t(0)
@@ -579,7 +663,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int t = 0; t < 2; ++t)
         if (ok && cnt[t] > 0) {
-          ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->q_full[t], items_of[t] & 1, err));
+          ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->q_full[t], (items_of[t] - (t == 1 ? q1_skipped : 0u)) & 1, err));
           ptx::tc_fence_after();
           if (ok) scores(t, 0, ptx::smem_u32(s_ring + stage * S::kTileBytes));
         }
@@ -592,33 +676,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         advance();
         ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->full[v_stage], v_phase, err));
         if (!ok) break;
-        // value rows behind the sequence's last key: zero, whatever the buffer holds there
-        const int valid = keys_left - j * kKeys;
         uint8_t* v_tile = s_ring + v_stage * S::kTileBytes;
-        if (valid < kKeys) {
-          for (int i = lane; i < (kKeys - valid) * 8; i += 32)
-#pragma unroll
-            for (int a = 0; a < S::kAtoms; ++a)
-              *reinterpret_cast<uint4*>(v_tile + a * 16384 + valid * 128 + i * 16) = make_uint4(0, 0, 0, 0);
-          ptx::fence_proxy_async_smem();
-          __syncwarp();
-        }
+        zero_tail(v_tile, keys_left - j * kKeys);
         const bool more = j + 1 < n;
         bool k_ready = false;
         const uint32_t v_addr = ptx::smem_u32(v_tile);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           if (!ok || j >= cnt[t]) continue;
-          ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->p_ready[t], p_uses[t] & 1, err));
-          ++p_uses[t];
-          if (ok && j == 0) ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->o_free[t], (items_of[t] & 1) ^ 1, err));
-          if (!ok) continue;
-          ptx::tc_fence_after();
-          {
-#pragma unroll
-            for (int k = 0; k < kKeys / 16; ++k)
-              ptx::umma_f16_ts_warp(tmem + 256 + t * D, tmem + t * 128 + k * 8, desc_v(v_addr + k * 2048), idesc_o, (j | k) != 0);
-          }
+          if (!(ok = weights_ready(t, j == 0))) continue;
+          values(t, v_addr, j == 0);
           if (j + 1 < cnt[t]) {
             if (!k_ready) {
               ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->full[stage], phase, err));
@@ -660,18 +727,31 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int row_pos = r / p.group, row_head = r % p.group;
     const int warp_pos = ((warp & 3) * 32) / p.group;
     const float c = p.scale_log2;
-    uint32_t s_uses = 0, items_done = 0;
+    uint32_t s_uses = 0, items_done = 0, others_done = 0, joins = 0;  // others_done: items of the other group
+    float2* ml = reinterpret_cast<float2*>(smem + S::kOffMl) + r;
     bool ok = true;
     while (true) {
       const Job* job = jobs.next(err);
       if (job == nullptr) break;
-      int n, rel, warp_rel;  // key tiles; keys that the row, and the warp's first row, see from the range's first on
+      // key tiles of this group; keys that the row, and the warp's first row, see from the range's first on;
+      // keys from one of the group's tiles to the next
+      int n, rel, warp_rel, stride = kKeys;
+      const bool shared = shared_item(p, job->it);
+      const int tq = shared ? 0 : t;  // query tile
+      bool other;                     // the other group has key tiles in this item
       {
         const Item& it = job->it;
-        n = tile_count(p, it, t);
-        const int pos = it.pos + t * p.tile_pos + row_pos;
+        n = tile_count(p, it, tq);
+        other = shared || tile_count(p, it, t ^ 1) > 0;
+        const int pos = it.pos + tq * p.tile_pos + row_pos;
         rel = (row_pos < p.tile_pos && pos < it.lq ? seen_keys(pos, it.lq, it.lk, p.causal) : 0) - it.t0 * kKeys;
-        warp_rel = seen_keys(min(it.pos + t * p.tile_pos + warp_pos, it.lq - 1), it.lq, it.lk, p.causal) - it.t0 * kKeys;
+        warp_rel = seen_keys(min(it.pos + tq * p.tile_pos + warp_pos, it.lq - 1), it.lq, it.lk, p.causal) - it.t0 * kKeys;
+        if (shared) {
+          n = (n + 1 - t) / 2;
+          rel -= t * kKeys;
+          warp_rel -= t * kKeys;
+          stride = 2 * kKeys;
+        }
       }
       float m = -INFINITY, mc = 0.f;
       float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
@@ -684,8 +764,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < 4; ++i) ptx::tmem_ld_32x32b_x32(t_s + i * 32, s[i]);
         ptx::tmem_wait_ld();
-        if ((j + 1) * kKeys > warp_rel) {  // some row of the warp does not see the whole tile
-          const int vis = rel - j * kKeys;
+        if (j * stride + kKeys > warp_rel) {  // some row of the warp does not see the whole tile
+          const int vis = rel - j * stride;
 #pragma unroll
           for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -751,7 +831,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) break;
       // ---- the item's rows of this tile
-      const float l = (sum0.x + sum0.y) + (sum1.x + sum1.y);
+      float l = (sum0.x + sum0.y) + (sum1.x + sum1.y);
       if (n > 0) {
         ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->o_full[t], items_done & 1, err));
         if (!ok) break;
@@ -759,66 +839,99 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const Item it = job->it;
       const int hk = job->hk;
+      if (shared && t == 1) {
+        // group 0 joins the two (the wait above also says that it has read the last item's)
+        *ml = make_float2(m, l);
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&bars->ml_ready);
+        ++items_done;
+        ++others_done;
+        jobs.done();
+        continue;
+      }
+      float f0 = 1.f, f1 = 0.f;  // factors of O_t and, in a shared item, of group 1's O
+      if (shared) {
+        ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->ml_ready, joins & 1, err)) &&
+             __all_sync(0xffffffffu, ptx::mbar_wait(&bars->o_full[1], others_done & 1, err));
+        if (!ok) break;
+        ptx::tc_fence_after();
+        ++joins;
+        const float2 o = *ml;
+        const float top = max3_nan(m, o.x, o.x), tc = top == -INFINITY ? 0.f : top * c;
+        f0 = ex2(fmaf(m, c, -tc));
+        f1 = ex2(fmaf(o.x, c, -tc));
+        l = f0 * l + f1 * o.y;
+        m = top;
+      }
       const int head = hk * p.group + row_head, pos = it.pos + t * p.tile_pos + row_pos;
       const bool live = row_pos < p.tile_pos && pos < it.lq;
       const int seen = live ? seen_keys(pos, it.lq, it.lk, p.causal) : 0;
-      if (it.slot < 0) {
-        const float inv = seen > 0 ? 1.f / l : 0.f;
-        T* dst = static_cast<T*>(p.out) + (long long)(it.q_row + pos) * p.ldo + head * D;
-        float bad = 0.f;
+      const float inv = it.slot >= 0 ? 1.f : seen > 0 ? 1.f / l : 0.f;
+      f0 *= inv;
+      f1 *= inv;
+      const long long at = it.slot < 0 ? 0 : ((long long)it.slot * p.kv_heads + hk) * p.rows_cap + t * p.tile_pos * p.group + r;
+      T* dst = static_cast<T*>(p.out) + (long long)(it.q_row + pos) * p.ldo + head * D;
+      float* part = p.part_o + at * D;
+      float bad = 0.f;
+#pragma unroll 1
+      for (int i = 0; i < D; i += 32) {
+        uint32_t o[32];
+        if (n > 0) {
+          ptx::tmem_ld_32x32b_x32(t_o + i, o);
+          ptx::tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-          uint32_t o[32];
-          if (n > 0) {
-            ptx::tmem_ld_32x32b_x32(t_o + i * 32, o);
-            ptx::tmem_wait_ld();
-          }
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f0);
+          if (shared) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const float x = seen > 0 ? __uint_as_float(o[e]) * inv : 0.f;
-            bad = fmaf(x, 0.f, bad);  // NaN as soon as one value is not finite
-            o[e] = __float_as_uint(x);
-          }
-          if (live) {
+            for (int h = 0; h < 2; ++h) {
+              uint32_t u[16];
+              ptx::tmem_ld_32x32b_x16(t_o + D + i + h * 16, u);
+              ptx::tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t* w = o + e * 8;
-              *reinterpret_cast<uint4*>(dst + i * 32 + e * 8) =
-                  make_uint4(E::pack(__uint_as_float(w[0]), __uint_as_float(w[1])), E::pack(__uint_as_float(w[2]), __uint_as_float(w[3])),
-                             E::pack(__uint_as_float(w[4]), __uint_as_float(w[5])), E::pack(__uint_as_float(w[6]), __uint_as_float(w[7])));
+              for (int e = 0; e < 16; ++e)
+                o[h * 16 + e] = __float_as_uint(fmaf(f1, __uint_as_float(u[e]), __uint_as_float(o[h * 16 + e])));
             }
           }
         }
-        uint32_t again = __ballot_sync(0xffffffffu, live && bad != 0.f);
+        if (n == 0 || (it.slot < 0 && seen == 0)) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0u;
+        }
+        if (live && it.slot < 0) {
+          uint32_t w[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float a = __uint_as_float(o[2 * e]), b = __uint_as_float(o[2 * e + 1]);
+            bad = fmaf(a, 0.f, fmaf(b, 0.f, bad));  // NaN as soon as one value is not finite
+            w[e] = E::pack(a, b);
+          }
+#pragma unroll
+          for (int e = 0; e < 16; e += 4) *reinterpret_cast<uint4*>(dst + i + e * 2) = make_uint4(w[e], w[e + 1], w[e + 2], w[e + 3]);
+        } else if (live) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(part + i + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        }
+      }
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (n > 0) {
+        if (lane == 0) {
+          ptx::mbar_arrive(&bars->o_free[t]);
+          if (shared) ptx::mbar_arrive(&bars->o_free[1]);
+        }
+        ++items_done;
+      }
+      if (other) ++others_done;
+      if (it.slot >= 0) {
+        if (live) p.part_ml[at] = make_float2(m, l);
+      } else {
+        uint32_t again = __ballot_sync(0xffffffffu, bad != 0.f);
         while (again != 0) {  // rare: a result that is not finite
           const int src = __ffs(again) - 1;
           again &= again - 1;
           store_row_by_definition<T, D>(p, it.q_row, it.lq, it.k_row, it.lk, __shfl_sync(0xffffffffu, pos, src),
                                         __shfl_sync(0xffffffffu, head, src));
         }
-      } else {
-        const long long at = ((long long)it.slot * p.kv_heads + hk) * p.rows_cap + t * p.tile_pos * p.group + r;
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-          uint32_t o[32];
-          if (n > 0) {
-            ptx::tmem_ld_32x32b_x32(t_o + i * 32, o);
-            ptx::tmem_wait_ld();
-          }
-          if (live) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              *reinterpret_cast<uint4*>(p.part_o + at * D + i * 32 + e * 4) =
-                  n > 0 ? make_uint4(o[e * 4], o[e * 4 + 1], o[e * 4 + 2], o[e * 4 + 3]) : make_uint4(0, 0, 0, 0);
-          }
-        }
-        if (live) p.part_ml[at] = make_float2(m, l);
-      }
-      if (n > 0) {
-        ptx::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(&bars->o_free[t]);
-        ++items_done;
       }
       jobs.done();
     }
