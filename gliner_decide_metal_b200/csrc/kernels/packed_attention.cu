@@ -53,7 +53,7 @@ namespace {
 constexpr int kKeys = 128;       // keys of a tile
 constexpr int kThreads = 384;     // three warpgroups; two of the third's warps only take part in barriers
 constexpr int kRowRegs = 216, kIssueRegs = 72;  // 256 * 216 + 128 * 72 = 384 * 168, the launch's registers
-constexpr int kPlanThreads = 1024;
+constexpr int kPlanThreads = 512, kPlanCached = 1024;  // (sequences whose offsets the planner reads once)
 constexpr int kPlanSms = 148;    // the planner's unit of work (the workspace size depends on it)
 constexpr float kGrowth = 8.0f;  // log2 growth of a row's maximum that moves its reference
 
@@ -210,6 +210,7 @@ constexpr int kBuckets = 512;
 // and the split items. One CTA: a warp takes a sequence at a time, its lanes the items.
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(Params p) {
   __shared__ int hist[kBuckets];
+  __shared__ int4 cached[kPlanCached];
   __shared__ unsigned long long s_work;
   __shared__ int s_items, s_max, s_slots, s_splits;
   ptx::grid_launch_next();
@@ -221,6 +222,24 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(Params p) {
   }
   for (int i = threadIdx.x; i < kBuckets; i += kPlanThreads) hist[i] = 0;
   ptx::grid_wait();
+  for (int b = threadIdx.x; b < min(p.batch, kPlanCached); b += kPlanThreads) {
+    int4 s;
+    if (!sequence(p, b, true, s.x, s.y, s.z, s.w)) s.y = 0;
+    cached[b] = s;
+  }
+  // a sequence of no queries, or of bad offsets, has no items
+  auto lengths = [&](int b, bool report, int& q0, int& lq, int& k0, int& lk) {
+    if (b < kPlanCached) {
+      const int4 s = cached[b];
+      q0 = s.x;
+      lq = s.y;
+      k0 = s.z;
+      lk = s.w;
+    } else if (!sequence(p, b, report, q0, lq, k0, lk)) {
+      lq = 0;
+    }
+    return lq > 0;
+  };
   __syncthreads();
   auto tiles_of = [&](int pos, int lq, int lk) {
     return (seen_keys(min(pos + per_item, lq) - 1, lq, lk, p.causal) + kKeys - 1) / kKeys;
@@ -230,7 +249,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(Params p) {
     int items = 0, most = 0;
     for (int b = warp; b < p.batch; b += warps) {
       int q0, lq, k0, lk;
-      if (!sequence(p, b, lane == 0, q0, lq, k0, lk)) continue;
+      if (!lengths(b, lane == 0, q0, lq, k0, lk)) continue;
       const int n = (lq + per_item - 1) / per_item;
       for (int i = lane; i < n; i += 32) {
         const int t = tiles_of(i * per_item, lq, lk);
@@ -270,7 +289,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(Params p) {
   for (int pass = 0; pass < 2; ++pass) {
     for (int b = warp; b < p.batch; b += warps) {
       int q0, lq, k0, lk;
-      if (!sequence(p, b, false, q0, lq, k0, lk)) continue;
+      if (!lengths(b, false, q0, lq, k0, lk)) continue;
       const int n = (lq + per_item - 1) / per_item;
       for (int i = lane; i < n; i += 32) {
         const int t = tiles_of(i * per_item, lq, lk);
@@ -960,29 +979,35 @@ __global__ void __launch_bounds__(256) combine_kernel(const Params p) {
     if (row >= rows_per_item) continue;
     const int pos = it.pos + row / p.group, head = hk * p.group + row % p.group;
     if (pos >= it.lq) continue;
-    float m = -INFINITY;
-    for (int s = lane; s < it.n; s += 32) {
-      const float ms = p.part_ml[((long long)(it.slot + s) * p.kv_heads + hk) * p.rows_cap + row].x;
-      m = max3_nan(m, ms, ms);
-    }
+    // 32 splits at a time: a lane has one's reference and sum, every lane its columns of all of them
+    float m = -INFINITY, l = 0.f, acc[PER] = {};
+    for (int s0 = 0; s0 < it.n; s0 += 32) {
+      const int count = min(32, it.n - s0);
+      const long long first = ((long long)(it.slot + s0) * p.kv_heads + hk) * p.rows_cap + row;
+      const long long step = (long long)p.kv_heads * p.rows_cap;
+      const float2 ml = lane < count ? p.part_ml[first + lane * step] : make_float2(-INFINITY, 0.f);
+      float top = max3_nan(m, ml.x, ml.x);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float u = __shfl_xor_sync(0xffffffffu, m, o);
-      m = max3_nan(m, u, u);
-    }
-    const float mc = m == -INFINITY ? 0.f : m * p.scale_log2;
-    float acc[PER] = {}, l = 0.f;
-    for (int s = 0; s < it.n; ++s) {
-      const long long at = ((long long)(it.slot + s) * p.kv_heads + hk) * p.rows_cap + row;
-      const float2 ml = p.part_ml[at];
-      const float f = ml.x == -INFINITY ? 0.f : ex2(fmaf(ml.x, p.scale_log2, -mc));
-      l = fmaf(f, ml.y, l);
-      const float* src = p.part_o + at * D + lane * PER;
+      for (int o = 16; o > 0; o >>= 1) {
+        const float u = __shfl_xor_sync(0xffffffffu, top, o);
+        top = max3_nan(top, u, u);
+      }
+      const float tc = top == -INFINITY ? 0.f : top * p.scale_log2;
+      const float old = ex2(fmaf(m, p.scale_log2, -tc)), f = ex2(fmaf(ml.x, p.scale_log2, -tc));
+      m = top;
+      l = fmaf(l, old, ptx::warp_sum(f * ml.y));
 #pragma unroll
-      for (int i = 0; i < PER; i += 2) {
-        const float2 v = *reinterpret_cast<const float2*>(src + i);
-        acc[i] = fmaf(f, v.x, acc[i]);
-        acc[i + 1] = fmaf(f, v.y, acc[i + 1]);
+      for (int i = 0; i < PER; ++i) acc[i] *= old;
+#pragma unroll 8
+      for (int s = 0; s < count; ++s) {
+        const float fs = __shfl_sync(0xffffffffu, f, s);
+        const float* src = p.part_o + (first + s * step) * D + lane * PER;
+#pragma unroll
+        for (int i = 0; i < PER; i += 2) {
+          const float2 v = *reinterpret_cast<const float2*>(src + i);
+          acc[i] = fmaf(fs, v.x, acc[i]);
+          acc[i + 1] = fmaf(fs, v.y, acc[i + 1]);
+        }
       }
     }
     const int seen = seen_keys(pos, it.lq, it.lk, p.causal);
