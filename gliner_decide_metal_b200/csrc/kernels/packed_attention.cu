@@ -122,6 +122,7 @@ struct Params {
   float* part_o;   // [slot * kv_heads + hk][rows_cap][D]
   float2* part_ml; // [slot * kv_heads + hk][rows_cap]
   int rows_cap, chunks_cap, splits_cap;
+  int wide_out;  // out's rows are 32-byte aligned
   int can_split;
   int* err;
 };
@@ -154,6 +155,22 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   float y;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
+}
+
+// 64 bytes of one row. A warp's rows lie in different lines, and the store unit takes a line at a time
+// whatever its width, so the widest stores cost least.
+__device__ __forceinline__ void store64(void* dst, const uint32_t (&w)[16], bool wide) {
+  if (wide) {
+#pragma unroll
+    for (int e = 0; e < 16; e += 8)
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(static_cast<uint32_t*>(dst) + e), "r"(w[e]),
+                   "r"(w[e + 1]), "r"(w[e + 2]), "r"(w[e + 3]), "r"(w[e + 4]), "r"(w[e + 5]), "r"(w[e + 6]), "r"(w[e + 7])
+                   : "memory");
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; e += 4)
+      *reinterpret_cast<uint4*>(static_cast<uint32_t*>(dst) + e) = make_uint4(w[e], w[e + 1], w[e + 2], w[e + 3]);
+  }
 }
 
 // One output row from memory over exactly its visible keys: plain softmax in fp32, one warp.
@@ -893,11 +910,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       float* part = p.part_o + at * D;
       float bad = 0.f;
 #pragma unroll 1
-      for (int i = 0; i < D; i += 32) {
+      for (int i = 0; i < D; i += 32) {  // (unrolled, its registers would spill into the key loop)
         uint32_t o[32];
         if (n > 0) {
           ptx::tmem_ld_32x32b_x32(t_o + i, o);
-          ptx::tmem_wait_ld();
+          ptx::tmem_wait_ld_of(o);
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f0);
           if (shared) {
@@ -905,7 +922,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int h = 0; h < 2; ++h) {
               uint32_t u[16];
               ptx::tmem_ld_32x32b_x16(t_o + D + i + h * 16, u);
-              ptx::tmem_wait_ld();
+              ptx::tmem_wait_ld_of(u);
 #pragma unroll
               for (int e = 0; e < 16; ++e)
                 o[h * 16 + e] = __float_as_uint(fmaf(f1, __uint_as_float(u[e]), __uint_as_float(o[h * 16 + e])));
@@ -924,11 +941,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             bad = fmaf(a, 0.f, fmaf(b, 0.f, bad));  // NaN as soon as one value is not finite
             w[e] = E::pack(a, b);
           }
-#pragma unroll
-          for (int e = 0; e < 16; e += 4) *reinterpret_cast<uint4*>(dst + i + e * 2) = make_uint4(w[e], w[e + 1], w[e + 2], w[e + 3]);
+          store64(dst + i, w, p.wide_out);
         } else if (live) {
-#pragma unroll
-          for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(part + i + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          store64(part + i, reinterpret_cast<const uint32_t(&)[16]>(o[0]), true);
+          store64(part + i + 16, reinterpret_cast<const uint32_t(&)[16]>(o[16]), true);
         }
       }
       ptx::tc_fence_before();
@@ -1098,6 +1114,7 @@ gdc_status launch_typed(const PackedAttentionArgs& a, cudaStream_t stream, int* 
   p.splits_cap = l.split ? int(l.items_ub) : 0;
   p.can_split = l.split;
   p.err = err;
+  p.wide_out = reinterpret_cast<uintptr_t>(a.out) % 32 == 0 && a.ldo % 16 == 0;
 
   static PerDeviceOnce configured;
   const cudaError_t ce = cudaError_t(per_device_once(configured, dev, [&] {
