@@ -12,6 +12,7 @@ namespace {
 constexpr int64_t kMaxRows = int64_t(1) << 30;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
 bool aligned2(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 1) == 0; }
 
 gdc_status check_elem(const char* what, gdc_dtype dtype, Elem* t) {
@@ -72,6 +73,8 @@ gdc_status gdc_packed_attention(gdc_dtype dtype, const void* q, int64_t ldq, con
   if (ldq % 8 || ldk % 8 || ldv % 8 || ldo % 8 || !aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out))
     return set_error(GDC_ERR_INVALID_INPUT,
                      "gdc_packed_attention: pointers must be 16-byte aligned and pitches multiples of 8");
+  if (!aligned4(q_off) || !aligned4(k_off))
+    return set_error(GDC_ERR_INVALID_INPUT, "gdc_packed_attention: offsets must be aligned to their type");
   if (std::max(std::max(ldq, ldo), std::max(ldk, ldv)) > (int64_t(1) << 31))
     return set_error(GDC_ERR_UNSUPPORTED, "gdc_packed_attention: row pitch above 2^31");
   const size_t need = packed_attention_workspace(batch, q_rows, k_rows, heads, kv_heads, head_dim);
@@ -101,8 +104,8 @@ gdc_status gdc_linear_residual(gdc_dtype dtype, const void* a, int64_t lda, cons
     return set_error(GDC_ERR_INVALID_INPUT, "gdc_linear_residual: a row pitch is below the row's width");
   if (lda % 8 || ldw % 8 || !aligned16(a) || !aligned16(w))
     return set_error(GDC_ERR_INVALID_INPUT, "gdc_linear_residual: a and w must be 16-byte aligned, their pitches multiples of 8");
-  if (!aligned2(bias) || !aligned2(residual) || !aligned2(out))
-    return set_error(GDC_ERR_INVALID_INPUT, "gdc_linear_residual: bias, residual and out must be aligned to their type");
+  if (!aligned2(bias) || !aligned2(residual) || !aligned2(out) || !aligned4(rows_dev))
+    return set_error(GDC_ERR_INVALID_INPUT, "gdc_linear_residual: bias, residual, out and rows_dev must be aligned to their type");
   if (std::max(std::max(lda, ldw), std::max(ldo, ldr)) > (int64_t(1) << 31))
     return set_error(GDC_ERR_UNSUPPORTED, "gdc_linear_residual: row pitch above 2^31");
   int* err = nullptr;
@@ -140,7 +143,7 @@ gdc_status gdc_gated_residual_norm(gdc_dtype dtype, const void* y, int64_t ldy, 
     return set_error(GDC_ERR_INVALID_INPUT, "gdc_gated_residual_norm: a row pitch is below cols");
   const void* all[] = {y, x, post_weight, post_bias, gate, pre_weight, pre_bias, x_out, n_out};
   for (const void* p : all)
-    if (!aligned2(p)) return set_error(GDC_ERR_INVALID_INPUT, "gdc_gated_residual_norm: pointers must be aligned to their type");
+    if (!aligned2(p) || !aligned4(rows_dev) || !aligned4(gate_index)) return set_error(GDC_ERR_INVALID_INPUT, "gdc_gated_residual_norm: pointers must be aligned to their type");
   if (std::max(std::max(ldy, ldx), std::max(ldxo, ldno)) > (int64_t(1) << 31))
     return set_error(GDC_ERR_UNSUPPORTED, "gdc_gated_residual_norm: row pitch above 2^31");
   int* err = nullptr;

@@ -53,7 +53,7 @@ namespace {
 constexpr int kKeys = 128;       // keys of a tile
 constexpr int kThreads = 384;     // three warpgroups; two of the third's warps only take part in barriers
 constexpr int kRowRegs = 216, kIssueRegs = 72;  // 256 * 216 + 128 * 72 = 384 * 168, the launch's registers
-constexpr int kPlanThreads = 512, kPlanCached = 1024;  // (sequences whose offsets the planner reads once)
+constexpr int kPlanThreads = 512;
 constexpr int kPlanSms = 148;    // the planner's unit of work (the workspace size depends on it)
 constexpr float kGrowth = 8.0f;  // log2 growth of a row's maximum that moves its reference
 
@@ -121,7 +121,8 @@ struct Params {
   SplitItem* splits;
   float* part_o;   // [slot * kv_heads + hk][rows_cap][D]
   float2* part_ml; // [slot * kv_heads + hk][rows_cap]
-  int rows_cap, chunks_cap, splits_cap;
+  int rows_cap, chunks_cap;
+  long long items_ub;
   int wide_out;  // out's rows are 32-byte aligned
   int can_split;
   int* err;
@@ -224,10 +225,10 @@ __device__ void store_row_by_definition(const Params& p, int q_row, int lq, int 
 constexpr int kBuckets = 512;
 
 // Lists the items by descending cost (key tiles of the chunk; a counting sort in shared memory)
-// and the split items. One CTA: a warp takes a sequence at a time, its lanes the items.
+// and the split items, in one CTA. Each warp has a run of sequences, a lane one of up to 32 at a time;
+// where a sequence has many items the lanes share them out.
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(Params p) {
   __shared__ int hist[kBuckets];
-  __shared__ int4 cached[kPlanCached];
   __shared__ unsigned long long s_work;
   __shared__ int s_items, s_max, s_slots, s_splits;
   ptx::grid_launch_next();
@@ -239,42 +240,39 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(Params p) {
   }
   for (int i = threadIdx.x; i < kBuckets; i += kPlanThreads) hist[i] = 0;
   ptx::grid_wait();
-  for (int b = threadIdx.x; b < min(p.batch, kPlanCached); b += kPlanThreads) {
-    int4 s;
-    if (!sequence(p, b, true, s.x, s.y, s.z, s.w)) s.y = 0;
-    cached[b] = s;
-  }
-  // a sequence of no queries, or of bad offsets, has no items
-  auto lengths = [&](int b, bool report, int& q0, int& lq, int& k0, int& lk) {
-    if (b < kPlanCached) {
-      const int4 s = cached[b];
-      q0 = s.x;
-      lq = s.y;
-      k0 = s.z;
-      lk = s.w;
-    } else if (!sequence(p, b, report, q0, lq, k0, lk)) {
-      lq = 0;
-    }
-    return lq > 0;
-  };
   __syncthreads();
-  auto tiles_of = [&](int pos, int lq, int lk) {
-    return (seen_keys(min(pos + per_item, lq) - 1, lq, lk, p.causal) + kKeys - 1) / kKeys;
+  const int run = (p.batch + warps - 1) / warps;  // sequences of a warp
+  // f(q0, lq, k0, lk, position, key tiles) for every item; a sequence of bad offsets has none
+  auto for_each_item = [&](bool report, auto&& f) {
+    const int last = min(p.batch, (warp + 1) * run);
+    for (int b0 = warp * run; b0 < last; b0 += 32) {
+      int q0 = 0, lq = 0, k0 = 0, lk = 0;
+      if (b0 + lane < last && !sequence(p, b0 + lane, report, q0, lq, k0, lk)) lq = 0;
+      const int n = (lq + per_item - 1) / per_item;
+      auto item = [&](int q, int l, int k, int m, int i) {
+        const int pos = i * per_item;
+        f(q, l, k, m, pos, (seen_keys(min(pos + per_item, l) - 1, l, m, p.causal) + kKeys - 1) / kKeys);
+      };
+      if (__reduce_max_sync(0xffffffffu, n) <= 4) {
+        for (int i = 0; i < n; ++i) item(q0, lq, k0, lk, i);
+      } else {
+        for (int s = 0; s < min(32, last - b0); ++s) {
+          const int q = __shfl_sync(0xffffffffu, q0, s), l = __shfl_sync(0xffffffffu, lq, s), k = __shfl_sync(0xffffffffu, k0, s),
+                    m = __shfl_sync(0xffffffffu, lk, s), ns = __shfl_sync(0xffffffffu, n, s);
+          for (int i = lane; i < ns; i += 32) item(q, l, k, m, i);
+        }
+      }
+    }
+    __syncwarp();
   };
   {
     unsigned long long work = 0;
     int items = 0, most = 0;
-    for (int b = warp; b < p.batch; b += warps) {
-      int q0, lq, k0, lk;
-      if (!lengths(b, lane == 0, q0, lq, k0, lk)) continue;
-      const int n = (lq + per_item - 1) / per_item;
-      for (int i = lane; i < n; i += 32) {
-        const int t = tiles_of(i * per_item, lq, lk);
-        work += t;
-        ++items;
-        most = max(most, t);
-      }
-    }
+    for_each_item(true, [&](int, int, int, int, int, int t) {
+      work += t;
+      ++items;
+      most = max(most, t);
+    });
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) work += __shfl_xor_sync(0xffffffffu, work, o);
     items = __reduce_add_sync(0xffffffffu, items);
@@ -286,7 +284,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(Params p) {
     }
   }
   __syncthreads();
-  // Chunk length. One round of chunks where the work allows short ones; otherwise about eight
+  // Chunk length (at most chunks_cap chunks a key head: their number is below work / length + items). One round of chunks where the work allows short ones; otherwise about eight
   // chunks an SM, none shorter than four tiles; at most chunks_cap chunks in all.
   int chunk = 1 << 30;
   if (p.can_split) {
@@ -303,33 +301,27 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(Params p) {
   int shift = 0;
   while ((min(chunk, s_max) >> shift) >= kBuckets) ++shift;
   auto bucket = [&](int tiles) { return kBuckets - 1 - min(kBuckets - 1, tiles >> shift); };
+  // More items than the query rows can hold: sequences overlap, so that some offset decreases, which has been
+  // reported; nothing is computed.
+  if (s_items > p.items_ub) {
+    if (threadIdx.x == 0) *p.header = PlanHeader{0, 0};
+    return;
+  }
   for (int pass = 0; pass < 2; ++pass) {
-    for (int b = warp; b < p.batch; b += warps) {
-      int q0, lq, k0, lk;
-      if (!lengths(b, false, q0, lq, k0, lk)) continue;
-      const int n = (lq + per_item - 1) / per_item;
-      for (int i = lane; i < n; i += 32) {
-        const int t = tiles_of(i * per_item, lq, lk);
-        const int parts = t > chunk ? (t + chunk - 1) / chunk : 1;
-        const int len = (t + parts - 1) / parts;
-        int slot = -1;
-        if (pass == 1 && parts > 1) {
-          // (the bounds can only be met by overlapping sequences, which some bad offset, reported
-          // above, leaves behind; their items are then dropped)
-          slot = atomicAdd(&s_slots, parts);
-          if (slot + parts > p.chunks_cap) continue;
-          const int at = atomicAdd(&s_splits, 1);
-          if (at >= p.splits_cap) continue;
-          p.splits[at] = SplitItem{q0, lq, k0, lk, i * per_item, slot, parts, 0};
-        }
-        for (int c = 0; c < parts; ++c) {
-          const int t0 = min(t, c * len), t1 = min(t, t0 + len);
-          const int at = atomicAdd(&hist[bucket(t1 - t0)], 1);
-          if (pass == 1 && at < p.chunks_cap)
-            p.items[at] = Item{q0, lq, k0, lk, i * per_item, t0, t1, parts > 1 ? slot + c : -1};
-        }
+    for_each_item(false, [&](int q0, int lq, int k0, int lk, int pos, int t) {
+      const int parts = t > chunk ? (t + chunk - 1) / chunk : 1;
+      const int len = (t + parts - 1) / parts;
+      int slot = -1;
+      if (pass == 1 && parts > 1) {
+        slot = atomicAdd(&s_slots, parts);
+        p.splits[atomicAdd(&s_splits, 1)] = SplitItem{q0, lq, k0, lk, pos, slot, parts, 0};
       }
-    }
+      for (int c = 0; c < parts; ++c) {
+        const int t0 = min(t, c * len), t1 = min(t, t0 + len);
+        const int at = atomicAdd(&hist[bucket(t1 - t0)], 1);
+        if (pass == 1) p.items[at] = Item{q0, lq, k0, lk, pos, t0, t1, parts > 1 ? slot + c : -1};
+      }
+    });
     __syncthreads();
     if (pass == 0) {
       // exclusive prefix sum of the histogram (descending cost: bucket 0 holds the longest)
@@ -350,8 +342,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(Params p) {
     }
   }
   if (threadIdx.x == 0) {
-    p.header->n_items = min(p.chunks_cap, hist[kBuckets - 1]);
-    p.header->n_splits = min(p.splits_cap, s_splits);
+    p.header->n_items = hist[kBuckets - 1];
+    p.header->n_splits = s_splits;
   }
 }
 
@@ -1111,7 +1103,7 @@ gdc_status launch_typed(const PackedAttentionArgs& a, cudaStream_t stream, int* 
   p.part_ml = reinterpret_cast<float2*>(a.workspace + l.part_ml_at);
   p.rows_cap = l.rows_cap;
   p.chunks_cap = l.chunks_cap;
-  p.splits_cap = l.split ? int(l.items_ub) : 0;
+  p.items_ub = l.items_ub;
   p.can_split = l.split;
   p.err = err;
   p.wide_out = reinterpret_cast<uintptr_t>(a.out) % 32 == 0 && a.ldo % 16 == 0;

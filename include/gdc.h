@@ -355,7 +355,8 @@ gdc_status gdc_linear(const uint16_t* a, const uint16_t* w, const uint16_t* bias
  *  kv_heads of at most 128 times it. scale is positive and finite.
  *  q_off, k_off: device int32 [batch + 1]; k_off NULL means q_off. Rows outside every sequence are
  *  neither read nor written. A sequence whose offsets decrease or leave [0, q_rows] or
- *  [0, k_rows] is skipped (its rows stay as they were) and reported.
+ *  [0, k_rows] is skipped (its rows stay as they were) and reported; where offsets that decrease
+ *  make other sequences overlap, those may be skipped too.
  *  workspace: device memory of gdc_packed_attention_workspace() bytes for the same sizes, 256-byte
  *  aligned, its contents arbitrary; calls that may run at the same time (graphs that share it
  *  too) need one each. */
