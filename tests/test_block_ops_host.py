@@ -33,7 +33,7 @@ NORM = dict(dtype=2, y=P, ldy=64, x=P, ldx=64, post_norm=1, post_weight=None, po
     (dict(scale=math.inf), INVALID), (dict(q=None), NULL), (dict(k=None), NULL), (dict(v=None), NULL), (dict(out=None), NULL),
     (dict(q_off=None), NULL), (dict(ldq=504), INVALID), (dict(ldk=120), INVALID), (dict(ldv=64), INVALID), (dict(ldo=8), INVALID),
     (dict(ldq=516), INVALID), (dict(ldk=132), INVALID), (dict(q=P + 2), INVALID), (dict(k=P + 8), INVALID), (dict(v=P + 4), INVALID),
-    (dict(out=P + 2), INVALID), (dict(workspace=None), NULL), (dict(workspace_bytes=0), INVALID), (dict(workspace=P + 16), INVALID),
+    (dict(out=P + 2), INVALID), (dict(q_off=P + 2), INVALID), (dict(k_off=P + 1), INVALID), (dict(workspace=None), NULL), (dict(workspace_bytes=0), INVALID), (dict(workspace=P + 16), INVALID),
     (dict(batch=0), OK), (dict(q_rows=0, q=None, out=None), OK)])
 def test_attention_refuses(change, status):
     assert _lib().gdc_packed_attention(*{**ATTENTION, **change}.values()) == status
@@ -56,7 +56,7 @@ def test_attention_workspace_query():
     (dict(act=-1), INVALID), (dict(a=None), NULL), (dict(w=None), NULL), (dict(out=None), NULL), (dict(lda=56), INVALID),
     (dict(ldw=56), INVALID), (dict(lda=68), INVALID), (dict(ldw=65), INVALID), (dict(ldr=99), INVALID), (dict(ldo=99), INVALID),
     (dict(a=P + 2), INVALID), (dict(w=P + 8), INVALID), (dict(bias=P + 1), INVALID), (dict(residual=P + 1), INVALID),
-    (dict(out=P + 1), INVALID), (dict(ldo=1 << 33), UNSUPPORTED), (dict(M=0, a=None), OK)])
+    (dict(out=P + 1), INVALID), (dict(rows_dev=P + 2), INVALID), (dict(ldo=1 << 33), UNSUPPORTED), (dict(M=0, a=None), OK)])
 def test_linear_refuses(change, status):
     assert _lib().gdc_linear_residual(*{**LINEAR, **change}.values()) == status
 
@@ -68,7 +68,8 @@ def test_linear_refuses(change, status):
     (dict(pre_norm=0), INVALID), (dict(pre_norm=0, n_out=None, x_out=None, y=None, gate=None, post_norm=0), NULL),
     (dict(gate_rows=0), INVALID), (dict(gate_rows=8), INVALID), (dict(gate=None, gate_index=P), INVALID),
     (dict(y=None), INVALID), (dict(y=None, gate=None), INVALID), (dict(ldy=63), INVALID), (dict(ldx=63), INVALID),
-    (dict(ldxo=63), INVALID), (dict(ldno=0), INVALID), (dict(x=P + 1), INVALID), (dict(gate=P + 1), INVALID), (dict(rows=0), OK)])
+    (dict(ldxo=63), INVALID), (dict(ldno=0), INVALID), (dict(x=P + 1), INVALID), (dict(gate=P + 1), INVALID),
+    (dict(gate_index=P + 2), INVALID), (dict(rows_dev=P + 1), INVALID), (dict(rows=0), OK)])
 def test_norm_refuses(change, status):
     assert _lib().gdc_gated_residual_norm(*{**NORM, **change}.values()) == status
 

@@ -283,6 +283,95 @@ def test_attention_two_streams_at_once():
     assert all(torch.equal(a, o) for a, o in zip(alone, outs))
 
 
+@pytest.mark.parametrize("dtype,dim", [("fp16", 64), ("bf16", 128)])
+def test_attention_output_pitch_and_alignment(dtype, dim):
+    """Outputs and inputs at 16-byte but not 32-byte addresses, with pitches above the width; what lies between
+    the rows stays."""
+    t = DTYPES[dtype][0]
+    heads, kv, lens = 4, 2, [150, 3]
+    n = sum(lens)
+    x = _normal(11, n * ((heads + 2 * kv) * dim + 24) + 8, dtype=t)[8:].view(n, -1)
+    q, k, v = x[:, :heads * dim], x[:, heads * dim + 8:(heads + kv) * dim + 8], x[:, (heads + kv) * dim + 16:(heads + 2 * kv) * dim + 16]
+    flat = torch.full((n * (heads * dim + 8) + 8,), 7.0, dtype=t, device="cuda")
+    out = flat[8:].view(n, heads * dim + 8)[:, :heads * dim]
+    off = _offsets(lens)
+    attention(q, k, v, off, None, heads, kv, True, out=out)
+    _done()
+    want, tol = attention_definition(q, k, v, off, None, heads, kv, True, np.float32(1 / math.sqrt(dim)).item(), out)
+    _within(out, want, tol)
+    assert (flat[8:].view(n, -1)[:, heads * dim:] == 7.0).all() and (flat[:8] == 7.0).all()
+
+
+def test_attention_without_any_keys():
+    q = _normal(12, 40, 256)
+    off = _offsets([33, 5], 1)
+    out = torch.full_like(q, 7.0)
+    ws = _workspace(2, 40, 0, 4, 4, 64)
+    zero = torch.zeros(3, dtype=torch.int32, device="cuda")
+    _check(_lib().gdc_packed_attention(2, q.data_ptr(), 256, None, 0, None, 0, out.data_ptr(), 256, off.data_ptr(), zero.data_ptr(), 2, 40, 0,
+                                       4, 4, 64, 1, 0.125, ws.data_ptr(), ws.numel(), _stream()))
+    _done()
+    assert (out[1:39] == 0).all() and (out[:1] == 7.0).all() and (out[39:] == 7.0).all()
+
+
+def test_attention_rows_beyond_32_bit_offsets():
+    """A key buffer of more than 2^31 elements: the last sequence lies behind that offset."""
+    width, rows = 4096, 600_000
+    kv = torch.zeros(rows, width, dtype=torch.float16, device="cuda")
+    at = rows - 700
+    kv[at:] = _normal(13, 700, width)
+    k, v = kv[:, 1024:1024 + 128], kv[:, width - 128:]
+    q = _normal(14, 3, 8 * 64)
+    qo = torch.tensor([0, 1, 3], dtype=torch.int32, device="cuda")
+    ko = torch.tensor([at, at + 500, rows], dtype=torch.int32, device="cuda")
+    got = attention(q, k, v, qo, ko, 8, 2, True)
+    _done()
+    want, tol = attention_definition(q, k, v, qo, ko, 8, 2, True, 0.125, torch.full_like(got, 7.0))
+    _within(got, want, tol)
+
+
+@pytest.mark.parametrize("batch,most", [(3000, 6), (700, 40), (40, 900)])
+def test_attention_many_sequences(batch, most):
+    rng = np.random.Generator(np.random.PCG64(batch))
+    lk = rng.integers(0, most, batch)
+    lq = np.minimum(lk, rng.integers(0, 3, batch))
+    _attention_case(15, "fp16", lq.tolist(), lk.tolist(), 4, 2, 64, True)
+
+
+def test_attention_refused_overlap_writes_nothing_out_of_place():
+    """Offsets that decrease and make later sequences overlap earlier ones: reported, rows outside every sequence
+    stay as they were."""
+    heads, dim, n = 8, 64, 512
+    q, k, v = (_normal(16 + i, n + 64, heads * dim) for i in range(3))
+    off = torch.tensor([0, n, 0, n, 0, n, 0, n], dtype=torch.int32, device="cuda")
+    got = attention(q, k, v, off, None, heads, heads, True)
+    torch.cuda.synchronize()
+    assert _lib().gdc_kernels_check_errors() == 3
+    assert (got[n:] == 7.0).all()
+
+
+def test_attention_shared_workspace_in_turn():
+    """Two captured calls on one workspace, replayed one after the other, again and again."""
+    dim, heads = 64, 4
+    cases, ws = [], _workspace(2, 2000, 6000, heads, heads, dim)
+    for n, (lq, lk) in enumerate((([900, 100], [900, 100]), ([1, 1], [5000, 700]))):
+        q, k, v = (_normal(17 + 3 * n + i, r, heads * dim) for i, r in enumerate((sum(lq), sum(lk), sum(lk))))
+        qo, ko = _offsets(lq), _offsets(lk)
+        alone = attention(q, k, v, qo, ko, heads, heads, True)
+        out = torch.empty_like(alone)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            attention(q, k, v, qo, ko, heads, heads, True, out=out, ws=ws)
+        cases.append((g, alone, out, (q, k, v, qo, ko)))
+    for _ in range(3):
+        for g, _, out, _ in cases:
+            out.fill_(7.0)
+            g.replay()
+    _done()
+    assert all(torch.equal(alone, out) for _, alone, out, _ in cases)
+
+
 # --------------------------------------------------------------------------------------- linear
 
 def linear(a, w, bias, residual, act, out=None, rows_dev=None):
@@ -411,6 +500,30 @@ def test_linear_captured_and_replayed():
     want, tol = linear_definition(a, w, None, x, 1)
     _within(out[:41], want[:41], tol[:41])
     assert (out[41:] == 7.0).all()
+
+
+@pytest.mark.parametrize("M", [300, 4000])
+def test_linear_rows_beyond_32_bit_offsets(M):
+    """Output rows further apart than 2^31 elements in all: the last ones lie behind that offset."""
+    pitch = 2 ** 31 // M + 4096
+    a, w, r = _normal(80, M, 64), _normal(81, 40, 64, std=0.2), _normal(82, M, 40)
+    flat = torch.empty(M * pitch, dtype=torch.float16, device="cuda")
+    out = flat.view(M, pitch)[:, :40]
+    out.copy_(r)
+    linear(a, w, None, out, 0, out=out)
+    _done()
+    _within(out, *linear_definition(a, w, None, r, 0))
+
+
+@pytest.mark.parametrize("M,N,K,act", [(64, 4096, 4096, 3), (256, 1024, 4096, 1), (2048, 4096, 1024, 1), (4885, 1024, 4096, 0), (3000, 2050, 520, 2),
+                                       (1, 8192, 8192, 0), (130, 130, 8192, 1)])
+def test_linear_forms_of_large_calls(M, N, K, act):
+    """Every form the choice of tiles comes to: split K, one round of wide tiles, several rounds."""
+    t = torch.bfloat16
+    a, w, b, r = _normal(83, M, K, dtype=t), _normal(84, N, K, std=1 / math.sqrt(K), dtype=t), _normal(85, N, dtype=t), _normal(86, M, N, dtype=t)
+    got = linear(a, w, b, r, act)
+    _done()
+    _within(got, *linear_definition(a, w, b, r, act))
 
 
 # ----------------------------------------------------------------------------------------- norm
@@ -580,6 +693,40 @@ def test_norm_spoiled_row_stays_alone():
     assert torch.isnan(got[1][[7, 21]]).all()
 
 
+@pytest.mark.parametrize("rows,cols", [(5000, 1024), (3000, 1001), (2500, 4096), (1500, 514), (700, 8200)])
+def test_norm_many_rows_in_place(rows, cols):
+    """More rows than the device holds at once, x and y overwritten row by row."""
+    y, x, pw, pb, g, nw, nb = _norm_inputs(98, rows, cols, "layer", "rms", 7, "fp16")
+    index = (torch.arange(rows, device="cuda") % 7).int()
+    full = (y, x, "layer", pw, pb, g, index, 0.5, "rms", nw, None, 1e-6)
+    want = norm_definition(*full)
+    xo, no = x.clone(), y.clone()
+    norm(no, xo, *full[2:], x_out=xo, n_out=no, rows_dev=torch.tensor([rows - 3], dtype=torch.int32, device="cuda"))
+    _done()
+    for o, (wt, tol), before in zip((xo, no), want, (x, y)):
+        _within(o[:-3], wt[:-3], tol[:-3])
+        assert torch.equal(o[-3:], before[-3:])
+
+
+def test_norm_captured_and_replayed():
+    y, x, pw, pb, g, nw, nb = _norm_inputs(99, 64, 384, "rms", "layer", 1, "bf16")
+    rows = torch.tensor([64], dtype=torch.int32, device="cuda")
+    args = (y, x, "rms", pw, None, g, None, 1.0, "layer", nw, nb, 1e-6)
+    xo, no = norm(*args, rows_dev=rows)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm(*args, x_out=xo, n_out=no, rows_dev=rows)
+    x.copy_(_normal(100, 64, 384, dtype=x.dtype))
+    rows.fill_(50)
+    xo.fill_(7.0), no.fill_(7.0)
+    graph.replay()
+    _done()
+    for o, (wt, tol) in zip((xo, no), norm_definition(*args)):
+        _within(o[:50], wt[:50], tol[:50])
+        assert (o[50:] == 7.0).all()
+
+
 # -------------------------------------------------------------------------------- a block of them
 
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
@@ -637,3 +784,66 @@ def test_a_block_over_packed_rows(dtype):
     g.replay()
     _done()
     verify()
+
+
+def test_calls_follow_each_other_without_waiting():
+    """Kernels that start before the one ahead of them has ended still read its results: a long chain of
+    dependent calls on one stream, each overwriting what the next reads, against the same chain with
+    a wait after every call."""
+    def chain(wait):
+        x = _normal(200, 96, 512)
+        w = [_normal(201 + i, 512, 512, std=0.04) for i in range(3)]
+        off = _offsets([40, 56])
+        ws = _workspace(2, 96, 96, 8, 8, 64)
+        h, y, c = (torch.empty_like(x) for _ in range(3))
+        for i in range(60):
+            norm(None, x, "none", None, None, None, None, 1.0, "rms", None, None, 1e-6, x_out=y, n_out=h)
+            wait()
+            linear(h, w[i % 3], None, None, 0, out=y)
+            wait()
+            attention(y, h, y, off, None, 8, 8, True, out=c, ws=ws)
+            wait()
+            linear(c, w[(i + 1) % 3], None, x, 3, out=x)
+            wait()
+        torch.cuda.synchronize()
+        return x
+    a, b = chain(lambda: None), chain(torch.cuda.synchronize)
+    _done()
+    assert torch.isfinite(a).all() and torch.equal(a, b)
+
+
+def test_first_use_of_a_kernel_inside_a_capture():
+    """Only the first call on a device has to come before a capture; a kernel first used inside one works."""
+    import subprocess
+    import sys
+    code = """
+import torch, sys
+sys.path.insert(0, {root!r})
+from tests import test_gpu_block_ops as t
+t.linear(t._normal(1, 8, 64), t._normal(2, 16, 64), None, None, 0)
+torch.cuda.synchronize()
+q = t._normal(3, 400, 512, dtype=torch.bfloat16)
+off = t._offsets([300, 100])
+ws = t._workspace(2, 400, 400, 4, 4, 128)
+outs = [torch.empty_like(q) for _ in range(3)]
+w = t._normal(4, 512, 512, std=0.04, dtype=torch.bfloat16)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    t.attention(q, q, q, off, None, 4, 4, True, out=outs[0], ws=ws)
+    t.linear(outs[0], w, None, q, 1, out=outs[1])
+    t.norm(outs[1], q, "rms", None, None, None, None, 1.0, "layer", None, None, 1e-6, x_out=outs[2], n_out=outs[0])
+g.replay()
+t._done()
+again = [torch.empty_like(q) for _ in range(3)]
+t.attention(q, q, q, off, None, 4, 4, True, out=again[0], ws=ws)
+t.linear(again[0], w, None, q, 1, out=again[1])
+t.norm(again[1], q, "rms", None, None, None, None, 1.0, "layer", None, None, 1e-6, x_out=again[2], n_out=again[0])
+t._done()
+assert all(torch.equal(a, b) for a, b in zip(outs, again))
+print("same")
+"""
+    from pathlib import Path
+    root = str(Path(__file__).resolve().parents[1])
+    r = subprocess.run([sys.executable, "-c", code.format(root=root)], capture_output=True, text=True, timeout=300, cwd=root)
+    assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]
