@@ -92,10 +92,14 @@ PlanLayout plan_layout(int batch, int64_t q_rows, int64_t k_rows, int heads, int
   l.items_ub = q_rows / per_item + std::min<int64_t>(batch, q_rows);
   l.rows_cap = int(std::min<int64_t>(int64_t(per_item) * G, q_rows * G));
   const int64_t jobs = l.items_ub * kv_heads;
-  // Splitting pays while there are few jobs to an SM; partial rows are bounded to 64 MB.
+  // Splitting pays while there are few jobs to an SM, the fewer the larger a partial result is (256 rows
+  // of 128 columns, written and read again, cost as much as three key tiles): at most eight jobs an SM up
+  // to 64 KB (1024 jobs of 256 x 64 over 32 key tiles: 261 us whole, 243 split), four at 128 KB. Partial
+  // rows are bounded to 64 MB.
   const int64_t row_bytes = int64_t(l.rows_cap) * (dim + 2) * 4;
   const int64_t cap = std::min<int64_t>((int64_t(64) << 20) / row_bytes, jobs + 8 * kPlanSms);
-  l.split = k_rows > 2 * kKeys && jobs <= 8 * kPlanSms && cap >= jobs + kPlanSms / 2;
+  const int64_t most = kPlanSms * std::max<int64_t>(2, std::min<int64_t>(8, 131072 / (int64_t(l.rows_cap) * dim)));
+  l.split = k_rows > 2 * kKeys && jobs <= most && cap >= jobs + kPlanSms / 2;
   l.planned = l.split || jobs > kPlanSms;
   l.chunks_cap = int(l.split ? cap / kv_heads : std::min<int64_t>(l.items_ub, INT32_MAX));
   auto up = [](size_t v) { return (v + 255) & ~size_t(255); };
@@ -112,7 +116,7 @@ struct Params {
   void* out;
   long long ldq, ldk, ldv, ldo;
   const int32_t *q_off, *k_off;
-  int batch, q_rows, k_rows, heads, kv_heads, group, tile_pos;  // tile_pos: positions of a tile
+  int batch, q_rows, k_rows, heads, kv_heads, dim, group, tile_pos;  // tile_pos: positions of a tile
   int causal;
   float scale, scale_log2;
   // plan
@@ -284,16 +288,23 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(Params p) {
     }
   }
   __syncthreads();
-  // Chunk length (at most chunks_cap chunks a key head: their number is below work / length + items). One round of chunks where the work allows short ones; otherwise about eight
-  // chunks an SM, none shorter than four tiles; at most chunks_cap chunks in all.
+  // Chunk length (at most chunks_cap chunks a key head: their number is below work / length + items).
+  // One round of chunks where the work allows short ones; otherwise about eight chunks an SM, none so
+  // short that its partial rows (which cost as much as `over` tiles) weigh much. Two sequences
+  // of 256 rows after 6000 keys: 103 us in chunks of four tiles, 77 to 86 us so; a prompt of 4096 tokens
+  // in 16 heads of 128: 99 us split, joining not counted, 74 us whole.
   int chunk = 1 << 30;
   if (p.can_split) {
     const long long work = (long long)s_work * p.kv_heads, jobs = (long long)s_items * p.kv_heads;
     auto ceil_div = [](long long a, long long b) { return (a + b - 1) / b; };
-    long long c = max(4ll, ceil_div(work, 8 * kPlanSms));
+    // rows * dim * 8 bytes at an SM's 44 bytes a nanosecond, over 1.9 us a tile
+    const long long over = p.rows_cap * p.dim / 10500;
+    long long c = max(4 + 8 * over, ceil_div(work, 8 * kPlanSms));
     if (jobs <= kPlanSms / 2) {
-      const long long one = max(2ll, ceil_div(work, kPlanSms - jobs));
-      if (one <= 8) c = one;
+      const long long one = max(2 + 2 * over, ceil_div(work, kPlanSms - jobs));
+      if (one <= 8 + 8 * over) c = one;
+    } else if (over > 1 && (long long)s_max * kPlanSms <= work + work / 4) {
+      c = chunk;  // the items even out by themselves
     }
     const long long room = (long long)p.chunks_cap * p.kv_heads - jobs;
     chunk = int(min((long long)chunk, max(c, ceil_div(work, max(1ll, room)))));
@@ -1091,6 +1102,7 @@ gdc_status launch_typed(const PackedAttentionArgs& a, cudaStream_t stream, int* 
   p.k_rows = int(a.k_rows);
   p.heads = a.heads;
   p.kv_heads = a.kv_heads;
+  p.dim = D;
   p.group = group;
   p.tile_pos = tile_pos;
   p.causal = a.causal;
