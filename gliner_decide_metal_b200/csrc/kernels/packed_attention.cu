@@ -871,13 +871,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) break;
       // ---- the item's rows of this tile
       float l = (sum0.x + sum0.y) + (sum1.x + sum1.y);
+      const Item it = job->it;
+      const int hk = job->hk;
+      const int head = hk * p.group + row_head, pos = it.pos + t * p.tile_pos + row_pos;
+      const bool live = row_pos < p.tile_pos && pos < it.lq;
+      const int seen = live ? seen_keys(pos, it.lq, it.lk, p.causal) : 0;
+      const long long at = it.slot < 0 ? 0 : ((long long)it.slot * p.kv_heads + hk) * p.rows_cap + t * p.tile_pos * p.group + r;
+      T* dst = static_cast<T*>(p.out) + (long long)(it.q_row + pos) * p.ldo + head * D;
+      float* part = p.part_o + at * D;
+      const bool scaled = it.slot < 0;  // a split's partial row is left unnormalised
+      // factors of O_t and, in a shared item, of group 1's O
+      float f0 = !scaled ? 1.f : seen > 0 ? 1.f / l : 0.f, f1 = 0.f;
       if (n > 0) {
         ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->o_full[t], items_done & 1, err));
         if (!ok) break;
         ptx::tc_fence_after();
       }
-      const Item it = job->it;
-      const int hk = job->hk;
       if (shared && t == 1) {
         // group 0 joins the two (the wait above also says that it has read the last item's)
         *ml = make_float2(m, l);
@@ -888,7 +897,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         jobs.done();
         continue;
       }
-      float f0 = 1.f, f1 = 0.f;  // factors of O_t and, in a shared item, of group 1's O
       if (shared) {
         ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->ml_ready, joins & 1, err)) &&
              __all_sync(0xffffffffu, ptx::mbar_wait(&bars->o_full[1], others_done & 1, err));
@@ -901,16 +909,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         f1 = ex2(fmaf(o.x, c, -tc));
         l = f0 * l + f1 * o.y;
         m = top;
+        const float inv = !scaled ? 1.f : seen > 0 ? 1.f / l : 0.f;
+        f0 *= inv;
+        f1 *= inv;
       }
-      const int head = hk * p.group + row_head, pos = it.pos + t * p.tile_pos + row_pos;
-      const bool live = row_pos < p.tile_pos && pos < it.lq;
-      const int seen = live ? seen_keys(pos, it.lq, it.lk, p.causal) : 0;
-      const float inv = it.slot >= 0 ? 1.f : seen > 0 ? 1.f / l : 0.f;
-      f0 *= inv;
-      f1 *= inv;
-      const long long at = it.slot < 0 ? 0 : ((long long)it.slot * p.kv_heads + hk) * p.rows_cap + t * p.tile_pos * p.group + r;
-      T* dst = static_cast<T*>(p.out) + (long long)(it.q_row + pos) * p.ldo + head * D;
-      float* part = p.part_o + at * D;
       float bad = 0.f;
 #pragma unroll 1
       for (int i = 0; i < D; i += 32) {  // (unrolled, its registers would spill into the key loop)
@@ -938,12 +940,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (live && it.slot < 0) {
           uint32_t w[16];
+          float2 not_finite[2] = {};  // NaN as soon as one value is not finite
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const float a = __uint_as_float(o[2 * e]), b = __uint_as_float(o[2 * e + 1]);
-            bad = fmaf(a, 0.f, fmaf(b, 0.f, bad));  // NaN as soon as one value is not finite
-            w[e] = E::pack(a, b);
+            const float2 a = make_float2(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1]));
+            not_finite[e & 1] = __ffma2_rn(a, make_float2(0.f, 0.f), not_finite[e & 1]);
+            w[e] = E::pack(a.x, a.y);
           }
+          bad += (not_finite[0].x + not_finite[0].y) + (not_finite[1].x + not_finite[1].y);
           store64(dst + i, w, p.wide_out);
         } else if (live) {
           store64(part + i, reinterpret_cast<const uint32_t(&)[16]>(o[0]), true);
