@@ -11,21 +11,24 @@
 // all heads of its group and a single token's G heads fill one tile. One work item is two such
 // tiles (256 rows) of one sequence and key head against a range of 128-key tiles.
 //
-// Roles of a CTA (one per SM, persistent over items):
+// Roles of a CTA (one per SM, persistent over items; each role waits for jobs from warp 9's ring):
 //   warps 0-3, 4-7  softmax of tile 0 / tile 1: one thread a row. Reads its 128 scores from TMEM,
 //                   writes the weights back over them as 16-bit MMA operands, and at an item's
 //                   end divides and stores the row (or stores the split's partial row).
 //   warp 8          issues the MMAs: S_t = Q_t K_j^T (both operands in shared memory), then
 //                   O_t += P_t V_j (P_t from TMEM); the tensor cores work on one tile while the
 //                   softmax warps work on the other.
-//   warp 9          TMA: Q tiles of the item and a ring of K and V tiles, running ahead into the
-//                   next item.
+//   warp 9          the CTA's jobs, and TMA: Q tiles of the item and a ring of K and V tiles, running
+//                   ahead into the next item.
 // TMEM: S_0 [0, 128), S_1 [128, 256), O_0 [256, 256 + D), O_1 behind it; P_t lies over S_t.
+// An item of one query tile (tokens taken one at a time) is shared by both row groups, which take
+// its key tiles in turn (shared_item).
 //
 // The reference m_i moves only when a row's maximum has grown by more than 2^8 (then the tile's
 // O rows are rescaled in TMEM): weights stay below 2^8, which 16-bit weights and fp32 sums hold
 // without loss, and most key tiles need no rescale. S_t(j) complete implies P_t V(j-1) complete
-// (one thread issues them in that order), so the rescale needs no wait of its own.
+// (one thread issues them in that order), so the rescale needs no wait of its own. The weights are
+// rounded to the tensors' type for the second product, the row's sum is of the unrounded ones.
 //
 // A value that no visible key contributes must not reach a row, but 0 * inf is NaN: a row whose
 // result is not finite is computed again from memory by one warp over exactly its visible keys
@@ -35,6 +38,19 @@
 // Plan. Lengths are device data. When there are more items than SMs, or few items with many keys,
 // plan_kernel lists the items, splits long key ranges into chunks (their partial rows are joined
 // by combine_kernel), and orders them by descending cost; otherwise a CTA finds its item itself.
+//
+// What bounds it, and what it reaches on a B200:
+//   prompts   256 rows x 128 keys at D = 128 take the tensor cores 2048 cycles and the exponential
+//             unit 2048, but a row group's chain (scores 1250 from its weights on, maximum 500,
+//             exponentials and rounding 1450, hand-over 300) takes 3550, and two groups fill it to
+//             1.7 times the longer of the two. 8192 tokens, 32 / 8 heads of 128, causal: 470 us,
+//             1170 TFLOP/s (545 us in a power-limited run of seconds). Tried and slower: part of the
+//             exponentials as polynomials, two threads a row, weights in halves signalled apart, two
+//             issuing warps, 64-key steps with two score buffers.
+//   D = 64    the tensor cores need half as long, the chain as long: 570 TFLOP/s.
+//   tokens    HBM: 48 tokens over 212,000 keys of 8 heads of 128: 155 us, 5.6 TB/s.
+//   short     32 sequences of 64 to 256 rows, 16 / 4 heads of 64: 31 us, of which 5 plan, 7 to 12 the
+//             first item of each CTA (its instructions are cold) and 4 to 5 each further one.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -531,230 +547,230 @@ __global__ void __launch_bounds__(kThreads, 1)
       Job job;
       const bool found = PLANNED || find_job(p, job);
       if (lane == 0) {
+        int stage = 0;
+        uint32_t phase = 0;
+        uint32_t q_uses[2] = {0, 0};
+        long long issued = 0;
+        bool ok = true;
+        for (int round = 0; ok; ++round) {
+          if (PLANNED)
+            job.more = next_planned(p, round, job);
+          else
+            job.more = found && round == 0;
+          Bars* b = bars;
+          if (!(ok = ptx::mbar_wait(&b->job_empty[round & 1], ((round >> 1) & 1) ^ 1, err))) break;
+          b->job[round & 1] = job;
+          ptx::mbar_arrive(&b->job_full[round & 1]);
+          if (!job.more) break;
+          const Item& it = job.it;
+          const int hk = job.hk;
+          const int n0 = tile_count(p, it, 0), n1 = tile_count(p, it, 1), n = max(n0, n1);
+          auto load_q = [&](int t) {
+            if (!(ok = ok && ptx::mbar_wait(&bars->q_empty[t], (q_uses[t] & 1) ^ 1, err))) return;
+            ++q_uses[t];
+            ptx::mbar_arrive_expect_tx(&bars->q_full[t], uint32_t(S::kAtoms * p.tile_pos * p.group * 128));
+            for (int a = 0; a < S::kAtoms; ++a)
+              ptx::tma_load_3d(s_q + t * S::kTileBytes + a * 16384, &tm_q, a * 64, hk * p.group,
+                               it.q_row + it.pos + t * p.tile_pos, &bars->q_full[t]);
+          };
+          auto load_kv = [&](const CUtensorMap* map, int j) {
+            if (!(ok = ok && ptx::mbar_wait(&bars->empty[stage], phase ^ 1, err))) return;
+            ptx::mbar_arrive_expect_tx(&bars->full[stage], uint32_t(S::kTileBytes));
+            for (int a = 0; a < S::kAtoms; ++a)
+              ptx::tma_load_2d(s_ring + stage * S::kTileBytes + a * 16384, map, hk * D + a * 64,
+                               it.k_row + (it.t0 + j) * kKeys, &bars->full[stage]);
+            ++issued;
+            if (++stage == S::kStages) {
+              stage = 0;
+              phase ^= 1;
+            }
+          };
+          if (n == 0) continue;
+          if (n0 > 0) load_q(0);
+          load_kv(&tm_k, 0);
+          if (n1 > 0) load_q(1);
+          const int ahead = shared_item(p, it) ? 2 : 1;  // key tiles before the first value tile
+          if (ahead == 2) load_kv(&tm_k, 1);
+          for (int j = 0; j < n && ok; ++j) {
+            load_kv(&tm_v, j);
+            if (j + ahead < n) load_kv(&tm_k, j + ahead);
+          }
+        }
+        // the loads in flight land before the CTA can exit (bounded)
+        auto landed = [&](uint64_t* bar, uint32_t parity) {
+          const unsigned long long t0 = ptx::globaltimer();
+          while (!ptx::mbar_try_wait(bar, parity) && ptx::globaltimer() - t0 < ptx::kTimeoutNs) {
+          }
+        };
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (q_uses[t] > 0) landed(&bars->q_full[t], (q_uses[t] - 1) & 1);
+        for (long long j = std::max(0ll, issued - S::kStages); j < issued; ++j)
+          landed(&bars->full[j % S::kStages], uint32_t((j / S::kStages) & 1));
+      }
+    }
+    if (warp == 8) {
+      constexpr uint32_t fmt = (E::kMmaFormat << 7) | (E::kMmaFormat << 10);
+      constexpr uint32_t idesc_s = ptx::idesc_f16_f32(128, kKeys) | fmt;
+      constexpr uint32_t idesc_o = ptx::idesc_f16_f32(128, D, 1) | fmt;
       int stage = 0;
       uint32_t phase = 0;
-      uint32_t q_uses[2] = {0, 0};
-      long long issued = 0;
+      uint32_t items_of[2] = {0, 0}, p_uses[2] = {0, 0};
+      uint32_t q1_skipped = 0;  // shared items: group 1 took part without a query tile of its own
       bool ok = true;
-      for (int round = 0; ok; ++round) {
-        if (PLANNED)
-          job.more = next_planned(p, round, job);
-        else
-          job.more = found && round == 0;
-        Bars* b = bars;
-        if (!(ok = ptx::mbar_wait(&b->job_empty[round & 1], ((round >> 1) & 1) ^ 1, err))) break;
-        b->job[round & 1] = job;
-        ptx::mbar_arrive(&b->job_full[round & 1]);
-        if (!job.more) break;
-        const Item& it = job.it;
-        const int hk = job.hk;
-        const int n0 = tile_count(p, it, 0), n1 = tile_count(p, it, 1), n = max(n0, n1);
-        auto load_q = [&](int t) {
-          if (!(ok = ok && ptx::mbar_wait(&bars->q_empty[t], (q_uses[t] & 1) ^ 1, err))) return;
-          ++q_uses[t];
-          ptx::mbar_arrive_expect_tx(&bars->q_full[t], uint32_t(S::kAtoms * p.tile_pos * p.group * 128));
-          for (int a = 0; a < S::kAtoms; ++a)
-            ptx::tma_load_3d(s_q + t * S::kTileBytes + a * 16384, &tm_q, a * 64, hk * p.group,
-                             it.q_row + it.pos + t * p.tile_pos, &bars->q_full[t]);
-        };
-        auto load_kv = [&](const CUtensorMap* map, int j) {
-          if (!(ok = ok && ptx::mbar_wait(&bars->empty[stage], phase ^ 1, err))) return;
-          ptx::mbar_arrive_expect_tx(&bars->full[stage], uint32_t(S::kTileBytes));
-          for (int a = 0; a < S::kAtoms; ++a)
-            ptx::tma_load_2d(s_ring + stage * S::kTileBytes + a * 16384, map, hk * D + a * 64,
-                             it.k_row + (it.t0 + j) * kKeys, &bars->full[stage]);
-          ++issued;
+      while (ok) {
+        const Job* job = jobs.next(err);
+        if (job == nullptr) break;
+        const int cnt[2] = {tile_count(p, job->it, 0), tile_count(p, job->it, 1)};
+        const int n = max(cnt[0], cnt[1]);
+        const int keys_left = job->it.lk - job->it.t0 * kKeys;
+        const bool shared = shared_item(p, job->it);
+        jobs.done();
+        if (n == 0) continue;
+        auto advance = [&] {
           if (++stage == S::kStages) {
             stage = 0;
             phase ^= 1;
           }
         };
-        if (n == 0) continue;
-        if (n0 > 0) load_q(0);
-        load_kv(&tm_k, 0);
-        if (n1 > 0) load_q(1);
-        const int ahead = shared_item(p, it) ? 2 : 1;  // key tiles before the first value tile
-        if (ahead == 2) load_kv(&tm_k, 1);
-        for (int j = 0; j < n && ok; ++j) {
-          load_kv(&tm_v, j);
-          if (j + ahead < n) load_kv(&tm_k, j + ahead);
-        }
-      }
-      // the loads in flight land before the CTA can exit (bounded)
-      auto landed = [&](uint64_t* bar, uint32_t parity) {
-        const unsigned long long t0 = ptx::globaltimer();
-        while (!ptx::mbar_try_wait(bar, parity) && ptx::globaltimer() - t0 < ptx::kTimeoutNs) {
-        }
-      };
+        // S_t = Q_tq K^T
+        auto products = [&](int t, int tq, uint32_t k_addr) {
+          const uint32_t q_addr = ptx::smem_u32(s_q + tq * S::kTileBytes);
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-        if (q_uses[t] > 0) landed(&bars->q_full[t], (q_uses[t] - 1) & 1);
-      for (long long j = std::max(0ll, issued - S::kStages); j < issued; ++j)
-        landed(&bars->full[j % S::kStages], uint32_t((j / S::kStages) & 1));
-      }
-    }
-    if (warp == 8) {
-    constexpr uint32_t fmt = (E::kMmaFormat << 7) | (E::kMmaFormat << 10);
-    constexpr uint32_t idesc_s = ptx::idesc_f16_f32(128, kKeys) | fmt;
-    constexpr uint32_t idesc_o = ptx::idesc_f16_f32(128, D, 1) | fmt;
-    int stage = 0;
-    uint32_t phase = 0;
-    uint32_t items_of[2] = {0, 0}, p_uses[2] = {0, 0};
-    uint32_t q1_skipped = 0;  // shared items: group 1 took part without a query tile of its own
-    bool ok = true;
-    while (ok) {
-      const Job* job = jobs.next(err);
-      if (job == nullptr) break;
-      const int cnt[2] = {tile_count(p, job->it, 0), tile_count(p, job->it, 1)};
-      const int n = max(cnt[0], cnt[1]);
-      const int keys_left = job->it.lk - job->it.t0 * kKeys;
-      const bool shared = shared_item(p, job->it);
-      jobs.done();
-      if (n == 0) continue;
-      auto advance = [&] {
-        if (++stage == S::kStages) {
-          stage = 0;
-          phase ^= 1;
-        }
-      };
-      // S_t = Q_tq K^T
-      auto products = [&](int t, int tq, uint32_t k_addr) {
-        const uint32_t q_addr = ptx::smem_u32(s_q + tq * S::kTileBytes);
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = uint32_t(k >> 2) * 16384 + (k & 3) * 32;
-          ptx::umma_f16_ss_warp(tmem + t * 128, ptx::desc_kmajor_sw128(q_addr + off), ptx::desc_kmajor_sw128(k_addr + off), idesc_s,
-                                k != 0);
-        }
-        ptx::umma_commit_warp(&bars->s_full[t]);
-      };
-      auto wait_tile = [&] {
-        const bool got = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->full[stage], phase, err));
-        ptx::tc_fence_after();
-        return got;
-      };
-      // value rows behind the sequence's last key (valid ones before them): zero, whatever the buffer holds there
-      auto zero_tail = [&](uint8_t* v_tile, int valid) {
-        if (valid >= kKeys) return;
-        for (int i = lane; i < (kKeys - valid) * 8; i += 32)
-#pragma unroll
-          for (int a = 0; a < S::kAtoms; ++a)
-            *reinterpret_cast<uint4*>(v_tile + a * 16384 + valid * 128 + i * 16) = make_uint4(0, 0, 0, 0);
-        ptx::fence_proxy_async_smem();
-        __syncwarp();
-      };
-      // O_t (+)= P_t V
-      auto values = [&](int t, uint32_t v_addr, bool first) {
-#pragma unroll
-        for (int k = 0; k < kKeys / 16; ++k)
-          ptx::umma_f16_ts_warp(tmem + 256 + t * D, tmem + t * 128 + k * 8, desc_v(v_addr + k * 2048), idesc_o, !first | (k != 0));
-      };
-      // the weights of P_t, and before its first product of an item, O_t's columns
-      auto weights_ready = [&](int t, bool first) {
-        bool got = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->p_ready[t], p_uses[t] & 1, err));
-        ++p_uses[t];
-        if (got && first) got = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->o_free[t], (items_of[t] & 1) ^ 1, err));
-        ptx::tc_fence_after();
-        return got;
-      };
-      if (shared) {
-        // tiles in the order K0 K1 V0 K2 V1 K3 ..., group j % 2 takes tile j
-        ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->q_full[0], items_of[0] & 1, err));
-        auto next_scores = [&](int t) {
-          ok = wait_tile();
-          if (!ok) return;
-          products(t, 0, ptx::smem_u32(s_ring + stage * S::kTileBytes));
-          ptx::umma_commit_warp(&bars->empty[stage]);
-          advance();
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t off = uint32_t(k >> 2) * 16384 + (k & 3) * 32;
+            ptx::umma_f16_ss_warp(tmem + t * 128, ptx::desc_kmajor_sw128(q_addr + off), ptx::desc_kmajor_sw128(k_addr + off), idesc_s,
+                                  k != 0);
+          }
+          ptx::umma_commit_warp(&bars->s_full[t]);
         };
-        if (ok) next_scores(0);
-        if (ok) next_scores(1);
-        if (ok && n == 2) ptx::umma_commit_warp(&bars->q_empty[0]);
-        for (int j = 0; j < n && ok; j += 2) {
+        auto wait_tile = [&] {
+          const bool got = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->full[stage], phase, err));
+          ptx::tc_fence_after();
+          return got;
+        };
+        // value rows behind the sequence's last key (valid ones before them): zero, whatever the buffer holds there
+        auto zero_tail = [&](uint8_t* v_tile, int valid) {
+          if (valid >= kKeys) return;
+          for (int i = lane; i < (kKeys - valid) * 8; i += 32)
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            if (!ok || j + t >= n) continue;
-            if (!(ok = wait_tile())) continue;
-            zero_tail(s_ring + stage * S::kTileBytes, keys_left - (j + t) * kKeys);
-            if (!(ok = weights_ready(t, j == 0))) continue;
-            values(t, ptx::smem_u32(s_ring + stage * S::kTileBytes), j == 0);
+            for (int a = 0; a < S::kAtoms; ++a)
+              *reinterpret_cast<uint4*>(v_tile + a * 16384 + valid * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+          ptx::fence_proxy_async_smem();
+          __syncwarp();
+        };
+        // O_t (+)= P_t V
+        auto values = [&](int t, uint32_t v_addr, bool first) {
+#pragma unroll
+          for (int k = 0; k < kKeys / 16; ++k)
+            ptx::umma_f16_ts_warp(tmem + 256 + t * D, tmem + t * 128 + k * 8, desc_v(v_addr + k * 2048), idesc_o, !first | (k != 0));
+        };
+        // the weights of P_t, and before its first product of an item, O_t's columns
+        auto weights_ready = [&](int t, bool first) {
+          bool got = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->p_ready[t], p_uses[t] & 1, err));
+          ++p_uses[t];
+          if (got && first) got = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->o_free[t], (items_of[t] & 1) ^ 1, err));
+          ptx::tc_fence_after();
+          return got;
+        };
+        if (shared) {
+          // tiles in the order K0 K1 V0 K2 V1 K3 ..., group j % 2 takes tile j
+          ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->q_full[0], items_of[0] & 1, err));
+          auto next_scores = [&](int t) {
+            ok = wait_tile();
+            if (!ok) return;
+            products(t, 0, ptx::smem_u32(s_ring + stage * S::kTileBytes));
             ptx::umma_commit_warp(&bars->empty[stage]);
             advance();
-            if (j + t + 2 < n) {
-              next_scores(t);
-              if (ok && j + t + 3 == n) ptx::umma_commit_warp(&bars->q_empty[0]);
+          };
+          if (ok) next_scores(0);
+          if (ok) next_scores(1);
+          if (ok && n == 2) ptx::umma_commit_warp(&bars->q_empty[0]);
+          for (int j = 0; j < n && ok; j += 2) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              if (!ok || j + t >= n) continue;
+              if (!(ok = wait_tile())) continue;
+              zero_tail(s_ring + stage * S::kTileBytes, keys_left - (j + t) * kKeys);
+              if (!(ok = weights_ready(t, j == 0))) continue;
+              values(t, ptx::smem_u32(s_ring + stage * S::kTileBytes), j == 0);
+              ptx::umma_commit_warp(&bars->empty[stage]);
+              advance();
+              if (j + t + 2 < n) {
+                next_scores(t);
+                if (ok && j + t + 3 == n) ptx::umma_commit_warp(&bars->q_empty[0]);
+              } else {
+                ptx::umma_commit_warp(&bars->o_full[t]);
+              }
+            }
+          }
+          ++items_of[0];
+          ++items_of[1];
+          ++q1_skipped;
+          continue;
+        }
+        auto scores = [&](int t, int j, uint32_t k_addr) {
+          products(t, t, k_addr);
+          if (j + 1 == cnt[t]) ptx::umma_commit_warp(&bars->q_empty[t]);
+        };
+        // S_t(0)
+        ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->full[stage], phase, err));
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (ok && cnt[t] > 0) {
+            ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->q_full[t], (items_of[t] - (t == 1 ? q1_skipped : 0u)) & 1, err));
+            ptx::tc_fence_after();
+            if (ok) scores(t, 0, ptx::smem_u32(s_ring + stage * S::kTileBytes));
+          }
+        if (!ok) break;
+        ptx::umma_commit_warp(&bars->empty[stage]);
+        advance();
+        for (int j = 0; j < n && ok; ++j) {
+          const int v_stage = stage;
+          const uint32_t v_phase = phase;
+          advance();
+          ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->full[v_stage], v_phase, err));
+          if (!ok) break;
+          uint8_t* v_tile = s_ring + v_stage * S::kTileBytes;
+          zero_tail(v_tile, keys_left - j * kKeys);
+          const bool more = j + 1 < n;
+          bool k_ready = false;
+          const uint32_t v_addr = ptx::smem_u32(v_tile);
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (!ok || j >= cnt[t]) continue;
+            if (!(ok = weights_ready(t, j == 0))) continue;
+            values(t, v_addr, j == 0);
+            if (j + 1 < cnt[t]) {
+              if (!k_ready) {
+                ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->full[stage], phase, err));
+                if (!ok) continue;
+                ptx::tc_fence_after();
+                k_ready = true;
+              }
+              scores(t, j + 1, ptx::smem_u32(s_ring + stage * S::kTileBytes));
             } else {
               ptx::umma_commit_warp(&bars->o_full[t]);
             }
           }
-        }
-        ++items_of[0];
-        ++items_of[1];
-        ++q1_skipped;
-        continue;
-      }
-      auto scores = [&](int t, int j, uint32_t k_addr) {
-        products(t, t, k_addr);
-        if (j + 1 == cnt[t]) ptx::umma_commit_warp(&bars->q_empty[t]);
-      };
-      // S_t(0)
-      ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->full[stage], phase, err));
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-        if (ok && cnt[t] > 0) {
-          ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->q_full[t], (items_of[t] - (t == 1 ? q1_skipped : 0u)) & 1, err));
-          ptx::tc_fence_after();
-          if (ok) scores(t, 0, ptx::smem_u32(s_ring + stage * S::kTileBytes));
-        }
-      if (!ok) break;
-      ptx::umma_commit_warp(&bars->empty[stage]);
-      advance();
-      for (int j = 0; j < n && ok; ++j) {
-        const int v_stage = stage;
-        const uint32_t v_phase = phase;
-        advance();
-        ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->full[v_stage], v_phase, err));
-        if (!ok) break;
-        uint8_t* v_tile = s_ring + v_stage * S::kTileBytes;
-        zero_tail(v_tile, keys_left - j * kKeys);
-        const bool more = j + 1 < n;
-        bool k_ready = false;
-        const uint32_t v_addr = ptx::smem_u32(v_tile);
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (!ok || j >= cnt[t]) continue;
-          if (!(ok = weights_ready(t, j == 0))) continue;
-          values(t, v_addr, j == 0);
-          if (j + 1 < cnt[t]) {
-            if (!k_ready) {
-              ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->full[stage], phase, err));
-              if (!ok) continue;
-              ptx::tc_fence_after();
-              k_ready = true;
-            }
-            scores(t, j + 1, ptx::smem_u32(s_ring + stage * S::kTileBytes));
-          } else {
-            ptx::umma_commit_warp(&bars->o_full[t]);
+          if (!ok) break;
+          ptx::umma_commit_warp(&bars->empty[v_stage]);
+          if (more) {
+            ptx::umma_commit_warp(&bars->empty[stage]);
+            advance();
           }
         }
-        if (!ok) break;
-        ptx::umma_commit_warp(&bars->empty[v_stage]);
-        if (more) {
-          ptx::umma_commit_warp(&bars->empty[stage]);
-          advance();
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (cnt[t] > 0) ++items_of[t];
+      }
+      // every issued MMA is done before TMEM is released
+      ptx::umma_commit_warp(&bars->drain);
+      if (lane == 0) {
+        const unsigned long long t0 = ptx::globaltimer();
+        while (!ptx::mbar_try_wait(&bars->drain, 0) && ptx::globaltimer() - t0 < ptx::kTimeoutNs) {
         }
       }
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-        if (cnt[t] > 0) ++items_of[t];
-    }
-    // every issued MMA is done before TMEM is released
-    ptx::umma_commit_warp(&bars->drain);
-    if (lane == 0) {
-      const unsigned long long t0 = ptx::globaltimer();
-      while (!ptx::mbar_try_wait(&bars->drain, 0) && ptx::globaltimer() - t0 < ptx::kTimeoutNs) {
-      }
-    }
     }
     __syncwarp();
   } else {
