@@ -20,14 +20,16 @@
 //                   softmax warps work on the other.
 //   warp 9          the CTA's jobs, and TMA: Q tiles of the item and a ring of K and V tiles, running
 //                   ahead into the next item.
-// TMEM: S_0 [0, 128), S_1 [128, 256), O_0 [256, 256 + D), O_1 behind it; P_t lies over S_t.
+// TMEM: S_0 [0, 128), S_1 [128, 256), O_0 [256, 256 + D), O_1 behind it; P_t lies over S_t at D = 128 and
+// behind the O's at D = 64, where S_t(j + 1) can then be computed beside the softmax of S_t(j).
 // An item of one query tile (tokens taken one at a time) is shared by both row groups, which take
 // its key tiles in turn (shared_item).
 //
 // The reference m_i moves only when a row's maximum has grown by more than 2^8 (then the tile's
 // O rows are rescaled in TMEM): weights stay below 2^8, which 16-bit weights and fp32 sums hold
 // without loss, and most key tiles need no rescale. S_t(j) complete implies P_t V(j-1) complete
-// (one thread issues them in that order), so the rescale needs no wait of its own. The weights are
+// (one thread issues them in that order) at D = 128, so the rescale needs no wait of its own; at D = 64
+// the row warps wait for P_t V(j-1) before they write O_t or P_t. The weights are
 // rounded to the tensors' type for the second product, the row's sum is of the unrounded ones.
 //
 // A value that no visible key contributes must not reach a row, but 0 * inf is NaN: a row whose
@@ -381,6 +383,10 @@ struct Shape {
   static constexpr int kAtoms = D / 64;
   static constexpr int kTileBytes = 128 * D * 2;
   static constexpr int kStages = D == 128 ? 5 : 10;
+  // D = 64 leaves TMEM columns for the weights beside the scores, so S_t(j + 1) is on its way while the
+  // softmax of S_t(j) is; at D = 128 the weights lie over the scores they come from.
+  static constexpr bool kOwnP = D == 64;
+  static constexpr int kAhead = kOwnP ? 2 : 1;  // key tiles before an item's first value tile
   static constexpr int kOffQ = 0;
   static constexpr int kOffRing = 2 * kTileBytes;
   static constexpr int kOffBar = kOffRing + kStages * kTileBytes;
@@ -391,7 +397,7 @@ struct Shape {
 
 struct Bars {
   uint64_t full[10], empty[10];
-  uint64_t q_full[2], q_empty[2], s_full[2], p_ready[2], o_full[2], o_free[2], drain;
+  uint64_t q_full[2], q_empty[2], s_full[2], p_ready[2], o_full[2], o_free[2], s_free[2], drain;
   uint64_t job_full[2], job_empty[2], ml_ready;
   uint32_t tmem, pad;
   Job job[2];
@@ -521,6 +527,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       ptx::mbar_init(&bars->p_ready[t], 4);
       ptx::mbar_init(&bars->o_full[t], 1);
       ptx::mbar_init(&bars->o_free[t], 4);
+      ptx::mbar_init(&bars->s_free[t], 4);
     }
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(&bars->job_full[i], 1);
@@ -589,8 +596,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (n0 > 0) load_q(0);
           load_kv(&tm_k, 0);
           if (n1 > 0) load_q(1);
-          const int ahead = shared_item(p, it) ? 2 : 1;  // key tiles before the first value tile
-          if (ahead == 2) load_kv(&tm_k, 1);
+          const int ahead = shared_item(p, it) ? 2 : S::kAhead;
+          if (ahead == 2 && n > 1) load_kv(&tm_k, 1);
           for (int j = 0; j < n && ok; ++j) {
             load_kv(&tm_v, j);
             if (j + ahead < n) load_kv(&tm_k, j + ahead);
@@ -659,11 +666,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           ptx::fence_proxy_async_smem();
           __syncwarp();
         };
-        // O_t (+)= P_t V
-        auto values = [&](int t, uint32_t v_addr, bool first) {
+        // O_t (+)= P_t V; o_full: of the item's last one, or where the weights have columns of their own of each
+        auto values = [&](int t, uint32_t v_addr, bool first, bool last) {
 #pragma unroll
           for (int k = 0; k < kKeys / 16; ++k)
-            ptx::umma_f16_ts_warp(tmem + 256 + t * D, tmem + t * 128 + k * 8, desc_v(v_addr + k * 2048), idesc_o, !first | (k != 0));
+            ptx::umma_f16_ts_warp(tmem + 256 + t * D, tmem + (S::kOwnP ? 384 + t * 64 : t * 128) + k * 8, desc_v(v_addr + k * 2048),
+                                  idesc_o, !first | (k != 0));
+          if (S::kOwnP || last) ptx::umma_commit_warp(&bars->o_full[t]);
         };
         // the weights of P_t, and before its first product of an item, O_t's columns
         auto weights_ready = [&](int t, bool first) {
@@ -693,14 +702,12 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (!(ok = wait_tile())) continue;
               zero_tail(s_ring + stage * S::kTileBytes, keys_left - (j + t) * kKeys);
               if (!(ok = weights_ready(t, j == 0))) continue;
-              values(t, ptx::smem_u32(s_ring + stage * S::kTileBytes), j == 0);
+              values(t, ptx::smem_u32(s_ring + stage * S::kTileBytes), j == 0, j + t + 2 >= n);
               ptx::umma_commit_warp(&bars->empty[stage]);
               advance();
               if (j + t + 2 < n) {
                 next_scores(t);
                 if (ok && j + t + 3 == n) ptx::umma_commit_warp(&bars->q_empty[0]);
-              } else {
-                ptx::umma_commit_warp(&bars->o_full[t]);
               }
             }
           }
@@ -725,6 +732,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         ptx::umma_commit_warp(&bars->empty[stage]);
         advance();
+        // S_t's columns have been read (step p_uses[t] of this tile, counted over the items)
+        auto scores_read = [&](int t) {
+          const bool got = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->s_free[t], p_uses[t] & 1, err));
+          ptx::tc_fence_after();
+          return got;
+        };
+        if (S::kOwnP && n > 1) {
+          ok = wait_tile();
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            if (ok && cnt[t] > 1 && (ok = scores_read(t))) scores(t, 1, ptx::smem_u32(s_ring + stage * S::kTileBytes));
+          if (!ok) break;
+          ptx::umma_commit_warp(&bars->empty[stage]);
+          advance();
+        }
         for (int j = 0; j < n && ok; ++j) {
           const int v_stage = stage;
           const uint32_t v_phase = phase;
@@ -733,24 +755,23 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ok) break;
           uint8_t* v_tile = s_ring + v_stage * S::kTileBytes;
           zero_tail(v_tile, keys_left - j * kKeys);
-          const bool more = j + 1 < n;
+          const bool more = j + S::kAhead < n;
           bool k_ready = false;
           const uint32_t v_addr = ptx::smem_u32(v_tile);
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             if (!ok || j >= cnt[t]) continue;
             if (!(ok = weights_ready(t, j == 0))) continue;
-            values(t, v_addr, j == 0);
-            if (j + 1 < cnt[t]) {
+            values(t, v_addr, j == 0, j + 1 == cnt[t]);
+            if (j + S::kAhead < cnt[t]) {
               if (!k_ready) {
                 ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->full[stage], phase, err));
                 if (!ok) continue;
                 ptx::tc_fence_after();
                 k_ready = true;
               }
-              scores(t, j + 1, ptx::smem_u32(s_ring + stage * S::kTileBytes));
-            } else {
-              ptx::umma_commit_warp(&bars->o_full[t]);
+              if (S::kOwnP && !(ok = scores_read(t))) continue;
+              scores(t, j + S::kAhead, ptx::smem_u32(s_ring + stage * S::kTileBytes));
             }
           }
           if (!ok) break;
@@ -779,10 +800,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int r = (warp & 3) * 32 + lane;
     const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + t * 128 + lanes, t_o = tmem + 256 + t * D + lanes;
+    const uint32_t t_p = S::kOwnP ? tmem + 384 + t * 64 + lanes : t_s;
     const int row_pos = r / p.group, row_head = r % p.group;
     const int warp_pos = ((warp & 3) * 32) / p.group;
     const float c = p.scale_log2;
-    uint32_t s_uses = 0, items_done = 0, others_done = 0, joins = 0;  // others_done: items of the other group
+    uint32_t s_uses = 0, o_uses = 0, joins = 0;
     float2* ml = reinterpret_cast<float2*>(smem + S::kOffMl) + r;
     bool ok = true;
     while (true) {
@@ -793,11 +815,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       int n, rel, warp_rel, stride = kKeys;
       const bool shared = shared_item(p, job->it);
       const int tq = shared ? 0 : t;  // query tile
-      bool other;                     // the other group has key tiles in this item
       {
         const Item& it = job->it;
         n = tile_count(p, it, tq);
-        other = shared || tile_count(p, it, t ^ 1) > 0;
         const int pos = it.pos + tq * p.tile_pos + row_pos;
         rel = (row_pos < p.tile_pos && pos < it.lq ? seen_keys(pos, it.lq, it.lk, p.causal) : 0) - it.t0 * kKeys;
         warp_rel = seen_keys(min(it.pos + tq * p.tile_pos + warp_pos, it.lq - 1), it.lq, it.lk, p.causal) - it.t0 * kKeys;
@@ -819,6 +839,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < 4; ++i) ptx::tmem_ld_32x32b_x32(t_s + i * 32, s[i]);
         ptx::tmem_wait_ld();
+        if (S::kOwnP) {
+          ptx::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(&bars->s_free[t]);
+        }
         if (j * stride + kKeys > warp_rel) {  // some row of the warp does not see the whole tile
           const int vis = rel - j * stride;
 #pragma unroll
@@ -840,6 +865,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           m = top;
           mc = m == -INFINITY ? 0.f : m * c;
         } else {
+          if (S::kOwnP) {  // the last product has read the weights and written O
+            ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->o_full[t], o_uses & 1, err));
+            ++o_uses;
+            if (!ok) break;
+            ptx::tc_fence_after();
+          }
           const bool grow = !((top - m) * c <= kGrowth) && top != m;
           if (__any_sync(0xffffffffu, grow)) {
             const float f = grow ? ex2(m * c - top * c) : 1.f;
@@ -877,7 +908,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               sum0 = __fadd2_rn(sum0, x);
             w[e] = E::pack(x.x, x.y);
           }
-          ptx::tmem_st_32x32b_x16(t_s + i * 16, w);
+          ptx::tmem_st_32x32b_x16(t_p + i * 16, w);
         }
         ptx::tmem_wait_st();
         ptx::tc_fence_before();
@@ -899,23 +930,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       // factors of O_t and, in a shared item, of group 1's O
       float f0 = !scaled ? 1.f : seen > 0 ? 1.f / l : 0.f, f1 = 0.f;
       if (n > 0) {
-        ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->o_full[t], items_done & 1, err));
+        ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->o_full[t], o_uses & 1, err));
+        ++o_uses;
         if (!ok) break;
         ptx::tc_fence_after();
       }
       if (shared && t == 1) {
         // group 0 joins the two (the wait above also says that it has read the last item's)
         *ml = make_float2(m, l);
+        ptx::tc_fence_before();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(&bars->ml_ready);
-        ++items_done;
-        ++others_done;
         jobs.done();
         continue;
       }
       if (shared) {
-        ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->ml_ready, joins & 1, err)) &&
-             __all_sync(0xffffffffu, ptx::mbar_wait(&bars->o_full[1], others_done & 1, err));
+        ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->ml_ready, joins & 1, err));  // O_1 is complete too
         if (!ok) break;
         ptx::tc_fence_after();
         ++joins;
@@ -972,14 +1002,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       ptx::tc_fence_before();
       __syncwarp();
-      if (n > 0) {
-        if (lane == 0) {
-          ptx::mbar_arrive(&bars->o_free[t]);
-          if (shared) ptx::mbar_arrive(&bars->o_free[1]);
-        }
-        ++items_done;
+      if (n > 0 && lane == 0) {
+        ptx::mbar_arrive(&bars->o_free[t]);
+        if (shared) ptx::mbar_arrive(&bars->o_free[1]);
       }
-      if (other) ++others_done;
       if (it.slot >= 0) {
         if (live) p.part_ml[at] = make_float2(m, l);
       } else {
