@@ -49,9 +49,11 @@
 //             1170 TFLOP/s (545 us in a power-limited run of seconds). Tried and slower: part of the
 //             exponentials as polynomials, two threads a row, weights in halves signalled apart, two
 //             issuing warps, 64-key steps with two score buffers.
-//   D = 64    the tensor cores need half as long, the chain as long: 570 TFLOP/s.
+//   D = 64    S_t is ready when its group is: waits 300, scores 300, maximum 500, exponentials 1600, 3000 in
+//             all with both groups on the exponential unit. Four prompts of 4096, 16 / 4 heads: 216 us,
+//             635 TFLOP/s (242 us with the weights over the scores).
 //   tokens    HBM: 48 tokens over 212,000 keys of 8 heads of 128: 155 us, 5.6 TB/s.
-//   short     32 sequences of 64 to 256 rows, 16 / 4 heads of 64: 31 us, of which 5 plan, 7 to 12 the
+//   short     32 sequences of 64 to 256 rows, 16 / 4 heads of 64: 29 us, of which 5 plan, 7 to 12 the
 //             first item of each CTA (its instructions are cold) and 4 to 5 each further one.
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -110,10 +112,9 @@ PlanLayout plan_layout(int batch, int64_t q_rows, int64_t k_rows, int heads, int
   l.items_ub = q_rows / per_item + std::min<int64_t>(batch, q_rows);
   l.rows_cap = int(std::min<int64_t>(int64_t(per_item) * G, q_rows * G));
   const int64_t jobs = l.items_ub * kv_heads;
-  // Splitting pays while there are few jobs to an SM, the fewer the larger a partial result is (256 rows
-  // of 128 columns, written and read again, cost as much as three key tiles): at most eight jobs an SM up
-  // to 64 KB (1024 jobs of 256 x 64 over 32 key tiles: 261 us whole, 243 split), four at 128 KB. Partial
-  // rows are bounded to 64 MB.
+  // Splitting pays while there are few jobs to an SM (many even out by themselves), the fewer the larger a
+  // partial result is (256 rows of 128 columns, written and read again, cost as much as three key tiles):
+  // at most eight jobs an SM up to 64 KB, four at 128 KB. Partial rows are bounded to 64 MB.
   const int64_t row_bytes = int64_t(l.rows_cap) * (dim + 2) * 4;
   const int64_t cap = std::min<int64_t>((int64_t(64) << 20) / row_bytes, jobs + 8 * kPlanSms);
   const int64_t most = kPlanSms * std::max<int64_t>(2, std::min<int64_t>(8, 131072 / (int64_t(l.rows_cap) * dim)));
@@ -310,7 +311,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(Params p) {
   // One round of chunks where the work allows short ones; otherwise about eight chunks an SM, none so
   // short that its partial rows (which cost as much as `over` tiles) weigh much. Two sequences
   // of 256 rows after 6000 keys: 103 us in chunks of four tiles, 77 to 86 us so; a prompt of 4096 tokens
-  // in 16 heads of 128: 99 us split, joining not counted, 74 us whole.
+  // in 16 heads of 128: 99 us split, joining not counted, 74 us whole; prompts of 6000, 700 and 300 in 16
+  // heads of 64: 157 us split, 123 us whole.
   int chunk = 1 << 30;
   if (p.can_split) {
     const long long work = (long long)s_work * p.kv_heads, jobs = (long long)s_items * p.kv_heads;
@@ -321,7 +323,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(Params p) {
     if (jobs <= kPlanSms / 2) {
       const long long one = max(2 + 2 * over, ceil_div(work, kPlanSms - jobs));
       if (one <= 8 + 8 * over) c = one;
-    } else if (over > 1 && (long long)s_max * kPlanSms <= work + work / 4) {
+    } else if (over > 0 && (long long)s_max * kPlanSms <= work + work / 4) {
       c = chunk;  // the items even out by themselves
     }
     const long long room = (long long)p.chunks_cap * p.kv_heads - jobs;
