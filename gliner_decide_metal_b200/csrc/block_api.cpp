@@ -108,6 +108,8 @@ gdc_status gdc_linear_residual(gdc_dtype dtype, const void* a, int64_t lda, cons
     return set_error(GDC_ERR_INVALID_INPUT, "gdc_linear_residual: bias, residual, out and rows_dev must be aligned to their type");
   if (std::max(std::max(lda, ldw), std::max(ldo, ldr)) > (int64_t(1) << 31))
     return set_error(GDC_ERR_UNSUPPORTED, "gdc_linear_residual: row pitch above 2^31");
+  if (residual == out && ldr != ldo && M > 1)
+    return set_error(GDC_ERR_INVALID_INPUT, "gdc_linear_residual: a residual that is out needs its pitch");
   int* err = nullptr;
   GDC_TRY(device_error_word(&err));
   const LinearResidualArgs args{a, w, bias, residual, out, lda, ldw, ldr, ldo, M, rows_dev, N, K, act};
@@ -143,9 +145,13 @@ gdc_status gdc_gated_residual_norm(gdc_dtype dtype, const void* y, int64_t ldy, 
     return set_error(GDC_ERR_INVALID_INPUT, "gdc_gated_residual_norm: a row pitch is below cols");
   const void* all[] = {y, x, post_weight, post_bias, gate, pre_weight, pre_bias, x_out, n_out};
   for (const void* p : all)
-    if (!aligned2(p) || !aligned4(rows_dev) || !aligned4(gate_index)) return set_error(GDC_ERR_INVALID_INPUT, "gdc_gated_residual_norm: pointers must be aligned to their type");
+    if (!aligned2(p) || !aligned4(rows_dev) || !aligned4(gate_index))
+      return set_error(GDC_ERR_INVALID_INPUT, "gdc_gated_residual_norm: pointers must be aligned to their type");
   if (std::max(std::max(ldy, ldx), std::max(ldxo, ldno)) > (int64_t(1) << 31))
     return set_error(GDC_ERR_UNSUPPORTED, "gdc_gated_residual_norm: row pitch above 2^31");
+  if (rows > 1 && ((x_out == x && ldxo != ldx) || (n_out && n_out == y && ldno != ldy)))
+    return set_error(GDC_ERR_INVALID_INPUT, "gdc_gated_residual_norm: an output that is an input needs its pitch");
+  if (x_out && x_out == n_out) return set_error(GDC_ERR_INVALID_INPUT, "gdc_gated_residual_norm: x_out and n_out are the same");
   int* err = nullptr;
   GDC_TRY(device_error_word(&err));
   const GatedNormArgs a{y, x, post_norm != 0 ? post_weight : nullptr, post_norm != 0 ? post_bias : nullptr, gate,

@@ -348,7 +348,8 @@ gdc_status gdc_linear(const uint16_t* a, const uint16_t* w, const uint16_t* bias
  * h / (heads / kv_heads):
  *   out[i, h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * q[i, h] . k[j] - max)
  * A query that sees no key gives zeros. What a query does not see never reaches its output, not
- * even where it is infinite or NaN.
+ * even where it is infinite or NaN (a row whose result is not finite is computed again, one key
+ * at a time: some 50 ns a key).
  *  q, out: q_rows rows of heads * head_dim; k, v: k_rows rows of kv_heads * head_dim; row pitches
  *  ldq, ldk, ldv, ldo in elements (q, k and v may be column blocks of one projection's output).
  *  Pointers 16-byte aligned, pitches multiples of 8. head_dim is 64 or 128, heads a multiple of
@@ -387,7 +388,7 @@ gdc_status gdc_linear_residual(gdc_dtype dtype, const void* a, int64_t lda, cons
  * 1 = LayerNorm, 2 = RMSNorm, each over a row's cols values with `eps` added to the (biased)
  * variance or mean square, times weight, plus bias; NULL weight = 1, NULL bias = 0.
  *  y NULL: no block before (x_out = x; x_out may then be NULL). x_out may be x itself (same pitch),
- *  n_out may be y itself.
+ *  n_out may be y itself (same pitch).
  *  gate: [gate_rows, cols], rows cols apart, or NULL (= 1). gate_index (device int32 [rows]) names
  *  the gate row of every row; without it gate_rows is 1 (one row for all) or at least rows (one each).
  *  A row whose index is outside [0, gate_rows) is skipped and reported.

@@ -74,6 +74,14 @@ def test_norm_refuses(change, status):
     assert _lib().gdc_gated_residual_norm(*{**NORM, **change}.values()) == status
 
 
+def test_outputs_laid_over_inputs_at_another_pitch_are_refused():
+    norm = {**NORM, "x_out": 2 * P, "n_out": 3 * P, "x": 4 * P}
+    for change in (dict(x_out=4 * P, ldxo=72), dict(n_out=P, ldno=65), dict(n_out=2 * P)):
+        assert _lib().gdc_gated_residual_norm(*{**norm, **change}.values()) == INVALID
+        assert _lib().gdc_last_error()
+    assert _lib().gdc_linear_residual(*{**LINEAR, "ldo": 104}.values()) == INVALID
+
+
 def test_other_entry_points_still_refuse_the_new_type():
     """GDC_BFLOAT16 belongs to the block operators: a classify input of that type is refused."""
     from gliner_decide_metal_b200 import _lib as b

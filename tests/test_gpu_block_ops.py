@@ -196,6 +196,32 @@ def test_attention_growing_scores():
         _within(got, want, tol)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("rows", [1, 3, 200])
+def test_attention_growing_scores_of_a_sequences_last_rows(dim, rows):
+    """The same where one query tile's key tiles are taken in turn by both row groups, and in split ranges."""
+    heads, lk = 4, [1500, 100, 3000]
+    lq = [min(rows, n) for n in lk]
+    q = _normal(24, sum(lq), heads * dim).abs()
+    k = (_normal(25, sum(lk), 2 * dim).abs() * torch.cat([torch.linspace(0.05, 2, n, device="cuda") for n in lk])[:, None]).half()
+    v = _normal(26, sum(lk), 2 * dim)
+    qo, ko = _offsets(lq), _offsets(lk)
+    got = attention(q, k, v, qo, ko, heads, 2, True, 0.125)
+    _done()
+    want, tol = attention_definition(q, k, v, qo, ko, heads, 2, True, 0.125, torch.full_like(got, 7.0))
+    _within(got, want, tol)
+
+
+@pytest.mark.parametrize("dtype,dim", [("fp16", 64), ("bf16", 64), ("fp16", 128)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_attention_prompts_and_tokens_in_one_batch(dtype, dim, causal):
+    """Every SM takes items of one and of two query tiles, of one key tile and of many, in mixed order."""
+    rng = np.random.Generator(np.random.PCG64(23))
+    lk = rng.integers(1, 700, 90)
+    lq = np.where(rng.random(90) < 0.5, 1, np.minimum(lk, rng.integers(1, 400, 90)))
+    _attention_case(23, dtype, lq.tolist(), lk.tolist(), 8, 4, dim, causal, first=1, behind=2)
+
+
 @pytest.mark.parametrize("dtype,dim", [("fp16", 64), ("bf16", 128)])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 def test_attention_keeps_what_is_not_seen_out(dtype, dim, bad):
