@@ -223,6 +223,24 @@ def test_attention_prompts_and_tokens_in_one_batch(dtype, dim, causal):
 
 
 @pytest.mark.parametrize("dtype,dim", [("fp16", 64), ("bf16", 128)])
+@pytest.mark.parametrize("rows", [1, 60])
+def test_attention_keys_of_weight_zero_before_an_infinite_value(dtype, dim, rows):
+    """A row that an infinite value reaches keeps its other columns, although its first keys score -inf (weight 0)."""
+    n, t = 300, DTYPES[dtype][0]
+    q, k, v = _normal(27, rows, dim, dtype=t).abs(), _normal(28, n, dim, dtype=t), _normal(29, n, dim, dtype=t)
+    k[:40, 5] = -math.inf
+    v[100, 7] = math.inf
+    qo, ko = _offsets([rows]), _offsets([n])
+    got = attention(q, k, v, qo, ko, 1, 1, True)
+    _done()
+    assert (got[:, 7] == math.inf).all()
+    v[100, 7] = 0
+    want, tol = attention_definition(q, k, v, qo, ko, 1, 1, True, np.float32(1 / math.sqrt(dim)).item(), torch.full_like(got, 7.0))
+    cols = [c for c in range(dim) if c != 7]
+    _within(got[:, cols], want[:, cols], tol[:, cols])
+
+
+@pytest.mark.parametrize("dtype,dim", [("fp16", 64), ("bf16", 128)])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 def test_attention_keeps_what_is_not_seen_out(dtype, dim, bad):
     """Infinite and NaN keys and values reach exactly the queries that see them."""
