@@ -39,20 +39,22 @@
 //
 // Plan. Lengths are device data. When there are more items than SMs, or few items with many keys,
 // plan_kernel lists the items, splits long key ranges into chunks (their partial rows are joined
-// by combine_kernel), and orders them by descending cost; otherwise a CTA finds its item itself.
+// by combine_kernel), and orders them by descending cost; otherwise, and for small batches of single
+// tokens (plan_layout), a CTA finds its items itself.
 //
 // What bounds it, and what it reaches on a B200:
 //   prompts   256 rows x 128 keys at D = 128 take the tensor cores 2048 cycles and the exponential
 //             unit 2048, but a row group's chain (scores 1250 from its weights on, maximum 500,
 //             exponentials and rounding 1450, hand-over 300) takes 3550, and two groups fill it to
-//             1.7 times the longer of the two. 8192 tokens, 32 / 8 heads of 128, causal: 470 us,
-//             1170 TFLOP/s (545 us in a power-limited run of seconds). Tried and slower: part of the
+//             1.7 times the longer of the two. 8192 tokens, 32 / 8 heads of 128, causal: 456 to
+//             474 us, 1200 TFLOP/s (540 us in a power-limited run of seconds). Tried and slower: part of the
 //             exponentials as polynomials, two threads a row, weights in halves signalled apart, two
 //             issuing warps, 64-key steps with two score buffers.
 //   D = 64    S_t is ready when its group is: waits 300, scores 300, maximum 500, exponentials 1600, 3000 in
 //             all with both groups on the exponential unit. Four prompts of 4096, 16 / 4 heads: 216 us,
 //             635 TFLOP/s (242 us with the weights over the scores).
-//   tokens    HBM: 48 tokens over 212,000 keys of 8 heads of 128: 155 us, 5.6 TB/s.
+//   tokens    HBM: 48 tokens over 212,000 keys of 8 heads of 128: 155 us, 5.6 TB/s. One
+//             token over 8000: 18 us, of which 10 its keys and 3 the joining.
 //   short     32 sequences of 64 to 256 rows, 16 / 4 heads of 64: 29 us, of which 5 plan, 7 to 12 the
 //             first item of each CTA (its instructions are cold) and 4 to 5 each further one.
 #include <cuda.h>
@@ -101,7 +103,7 @@ struct PlanLayout {
   int64_t items_ub;    // upper bound of (sequence, item) pairs
   int rows_cap;        // rows of an item that can be used
   int chunks_cap;      // planned items per key head, splits included
-  bool planned, split;
+  bool planned, split;  // split and not planned: every CTA lists the ranges itself
   size_t items_at, splits_at, part_o_at, part_ml_at, bytes;
 };
 
@@ -119,7 +121,12 @@ PlanLayout plan_layout(int batch, int64_t q_rows, int64_t k_rows, int heads, int
   const int64_t cap = std::min<int64_t>((int64_t(64) << 20) / row_bytes, jobs + 8 * kPlanSms);
   const int64_t most = kPlanSms * std::max<int64_t>(2, std::min<int64_t>(8, 131072 / (int64_t(l.rows_cap) * dim)));
   l.split = k_rows > 2 * kKeys && jobs <= most && cap >= jobs + kPlanSms / 2;
-  l.planned = l.split || jobs > kPlanSms;
+  // Up to 128 sequences of one item each (tokens taken one at a time) and about 48 key tiles an SM: every CTA
+  // goes over the offsets itself, which spares a launch (one token over 8000 keys 22.1 -> 18.2 us, 32 over
+  // 1000 38.8 -> 35.1, 48 over 95,000 in all 92.7 -> 81.8). With more the planner's order by cost is worth it
+  // (48 over 212,000: 154 us planned, 166 so).
+  const bool direct = q_rows <= per_item && batch <= 128 && (k_rows / kKeys + batch) * kv_heads <= 48 * kPlanSms;
+  l.planned = l.split ? !direct : jobs > kPlanSms;
   l.chunks_cap = int(l.split ? cap / kv_heads : std::min<int64_t>(l.items_ub, INT32_MAX));
   auto up = [](size_t v) { return (v + 255) & ~size_t(255); };
   l.items_at = 256;
@@ -273,6 +280,31 @@ __device__ void store_row_by_definition(const Params& p, int q_row, int lq, int 
 
 // ------------------------------------------------------------------------------------- plan
 
+// Length of the chunks that key ranges are split into, in tiles (at most chunks_cap chunks a key head:
+// their number is below work / length + items; work, items and the longest item are of one key head).
+// One round of chunks where the work allows short ones; otherwise about eight chunks an SM, none so
+// short that its partial rows (which cost as much as `over` tiles) weigh much. Two sequences
+// of 256 rows after 6000 keys: 103 us in chunks of four tiles, 77 to 86 us so; a prompt of 4096 tokens
+// in 16 heads of 128: 99 us split, joining not counted, 74 us whole; prompts of 6000, 700 and 300 in 16
+// heads of 64: 157 us split, 123 us whole.
+template <typename I>
+__device__ __forceinline__ int chunk_length(const Params& p, I head_work, int items, int longest) {
+  constexpr I kSms = kPlanSms, kWhole = 1 << 30;
+  const I work = head_work * p.kv_heads, jobs = I(items) * p.kv_heads;
+  auto ceil_div = [](I a, I b) { return (a + b - 1) / b; };
+  // rows * dim * 8 bytes at an SM's 44 bytes a nanosecond, over 1.9 us a tile
+  const I over = p.rows_cap * p.dim / 10500;
+  I c = max(4 + 8 * over, ceil_div(work, 8 * kSms));
+  if (jobs <= kSms / 2) {
+    const I one = max(2 + 2 * over, ceil_div(work, kSms - jobs));
+    if (one <= 8 + 8 * over) c = one;
+  } else if (over > 0 && I(longest) * kSms <= work + work / 4) {
+    c = kWhole;  // the items even out by themselves
+  }
+  const I room = I(p.chunks_cap) * p.kv_heads - jobs;
+  return int(min(kWhole, max(c, ceil_div(work, max(I(1), room)))));
+}
+
 constexpr int kBuckets = 512;
 
 // Lists the items by descending cost (key tiles of the chunk; a counting sort in shared memory)
@@ -335,28 +367,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(Params p) {
     }
   }
   __syncthreads();
-  // Chunk length (at most chunks_cap chunks a key head: their number is below work / length + items).
-  // One round of chunks where the work allows short ones; otherwise about eight chunks an SM, none so
-  // short that its partial rows (which cost as much as `over` tiles) weigh much. Two sequences
-  // of 256 rows after 6000 keys: 103 us in chunks of four tiles, 77 to 86 us so; a prompt of 4096 tokens
-  // in 16 heads of 128: 99 us split, joining not counted, 74 us whole; prompts of 6000, 700 and 300 in 16
-  // heads of 64: 157 us split, 123 us whole.
-  int chunk = 1 << 30;
-  if (p.can_split) {
-    const long long work = (long long)s_work * p.kv_heads, jobs = (long long)s_items * p.kv_heads;
-    auto ceil_div = [](long long a, long long b) { return (a + b - 1) / b; };
-    // rows * dim * 8 bytes at an SM's 44 bytes a nanosecond, over 1.9 us a tile
-    const long long over = p.rows_cap * p.dim / 10500;
-    long long c = max(4 + 8 * over, ceil_div(work, 8 * kPlanSms));
-    if (jobs <= kPlanSms / 2) {
-      const long long one = max(2 + 2 * over, ceil_div(work, kPlanSms - jobs));
-      if (one <= 8 + 8 * over) c = one;
-    } else if (over > 0 && (long long)s_max * kPlanSms <= work + work / 4) {
-      c = chunk;  // the items even out by themselves
-    }
-    const long long room = (long long)p.chunks_cap * p.kv_heads - jobs;
-    chunk = int(min((long long)chunk, max(c, ceil_div(work, max(1ll, room)))));
-  }
+  const int chunk = p.can_split ? chunk_length<long long>(p, (long long)s_work, s_items, s_max) : 1 << 30;
   int shift = 0;
   while ((min(chunk, s_max) >> shift) >= kBuckets) ++shift;
   auto bucket = [&](int tiles) { return kBuckets - 1 - min(kBuckets - 1, tiles >> shift); };
@@ -475,6 +486,17 @@ __device__ __forceinline__ bool next_planned(const Params& p, int round, Job& jo
   return true;
 }
 
+// Inclusive sum over the warp's lanes up to this one.
+__device__ __forceinline__ int warp_prefix(int v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+
 // The unplanned job of this CTA: the (blockIdx.x / kv_heads)-th item in sequence order. One warp;
 // the result is the same in every lane.
 __device__ __forceinline__ bool find_job(const Params& p, Job& job) {
@@ -484,12 +506,7 @@ __device__ __forceinline__ bool find_job(const Params& p, Job& job) {
   for (int b0 = 0; b0 < p.batch; b0 += 32) {
     int q0 = 0, lq = 0, k0 = 0, lk = 0, n = 0;
     if (b0 + lane < p.batch && sequence(p, b0 + lane, true, q0, lq, k0, lk)) n = (lq + per_item - 1) / per_item;
-    int incl = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += u;
-    }
+    const int incl = warp_prefix(n);
     const int i = want - (incl - n);
     const uint32_t hit = __ballot_sync(0xffffffffu, i >= 0 && i < n);
     if (hit != 0) {
@@ -506,6 +523,74 @@ __device__ __forceinline__ bool find_job(const Params& p, Job& job) {
       return true;
     }
     want -= __shfl_sync(0xffffffffu, incl, 31);
+  }
+  return false;
+}
+
+// Calls whose sequences have an item each at most (split, not planned): sequence b of this lane, its key
+// tiles (-1: no item). One warp.
+__device__ __forceinline__ int only_item(const Params& p, int b, bool report, int& q0, int& lq, int& k0, int& lk) {
+  q0 = lq = k0 = lk = 0;
+  if (b >= p.batch || !sequence(p, b, report, q0, lq, k0, lk) || lq == 0) return -1;
+  return (seen_keys(lq - 1, lq, lk, p.causal) + kKeys - 1) / kKeys;
+}
+
+// The chunk length of such a call (0: nothing to do); CTA 0 lists the split items for combine_kernel.
+__device__ __forceinline__ int plan_in_place(const Params& p) {
+  const int lane = threadIdx.x & 31;
+  int work = 0, items = 0, longest = 0, q0, lq, k0, lk;
+  for (int b0 = 0; b0 < p.batch; b0 += 32) {
+    const int t = only_item(p, b0 + lane, true, q0, lq, k0, lk);
+    items += t >= 0;
+    work += max(t, 0);
+    longest = max(longest, t);
+  }
+  work = __reduce_add_sync(0xffffffffu, work);
+  items = __reduce_add_sync(0xffffffffu, items);
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  const bool none = items == 0 || items > p.items_ub;  // (overlapping sequences, as in plan_kernel)
+  const int chunk = none ? 0 : chunk_length<int>(p, work, items, longest);
+  if (blockIdx.x == 0) {
+    int splits = 0, slots = 0;
+    for (int b0 = 0; !none && b0 < p.batch; b0 += 32) {
+      const int t = only_item(p, b0 + lane, false, q0, lq, k0, lk);
+      const int parts = t > chunk ? (t + chunk - 1) / chunk : 0;
+      const uint32_t split = __ballot_sync(0xffffffffu, parts > 0);
+      const int incl = warp_prefix(parts);
+      if (parts > 0)
+        p.splits[splits + __popc(split & ((1u << lane) - 1))] = SplitItem{q0, lq, k0, lk, 0, slots + incl - parts, parts, 0};
+      splits += __popc(split);
+      slots += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (lane == 0) *p.header = PlanHeader{0, splits};
+  }
+  return chunk;
+}
+
+// The CTA's job of a round: its number counts the chunks of all sequences in order, every other round backwards.
+__device__ __forceinline__ bool find_chunk(const Params& p, int chunk, int round, Job& job) {
+  if (chunk == 0) return false;
+  const int lane = threadIdx.x & 31, g = gridDim.x;
+  const int at = round * g + ((round & 1) ? g - 1 - int(blockIdx.x) : int(blockIdx.x));
+  int want = at / p.kv_heads, slots = 0;
+  job.hk = at % p.kv_heads;
+  for (int b0 = 0; b0 < p.batch; b0 += 32) {
+    int q0, lq, k0, lk;
+    const int t = only_item(p, b0 + lane, false, q0, lq, k0, lk);
+    const int parts = t > chunk ? (t + chunk - 1) / chunk : int(t >= 0), slotted = parts > 1 ? parts : 0;
+    const int incl = warp_prefix(parts), slots_incl = warp_prefix(slotted);
+    const int i = want - (incl - parts);
+    const uint32_t hit = __ballot_sync(0xffffffffu, i >= 0 && i < parts);
+    if (hit != 0) {
+      const int len = parts > 0 ? (t + parts - 1) / parts : 0;
+      const int t0 = min(t, i * len), slot = parts > 1 ? slots + slots_incl - slotted + i : -1;
+      const int src = __ffs(hit) - 1;
+      auto of = [&](int v) { return __shfl_sync(0xffffffffu, v, src); };
+      job.it = Item{of(q0), of(lq), of(k0), of(lk), 0, of(t0), of(min(t, t0 + len)), of(slot)};
+      return true;
+    }
+    want -= __shfl_sync(0xffffffffu, incl, 31);
+    slots += __shfl_sync(0xffffffffu, slots_incl, 31);
   }
   return false;
 }
@@ -582,23 +667,27 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
     if (warp == 9) {
       Job job;
-      const bool found = PLANNED || find_job(p, job);
-      if (lane == 0) {
-        int stage = 0;
-        uint32_t phase = 0;
-        uint32_t q_uses[2] = {0, 0};
-        long long issued = 0;
+      int stage = 0;
+      uint32_t phase = 0;
+      uint32_t q_uses[2] = {0, 0};
+      long long issued = 0;
+      const int chunk = !PLANNED && p.can_split ? plan_in_place(p) : 0;
+      for (int round = 0;; ++round) {  // the warp finds a job, one lane hands it out and loads its tiles
+        bool more;
+        if (PLANNED)
+          more = next_planned(p, round, job);
+        else
+          more = p.can_split ? find_chunk(p, chunk, round, job) : round == 0 && find_job(p, job);
         bool ok = true;
-        for (int round = 0; ok; ++round) {
-          if (PLANNED)
-            job.more = next_planned(p, round, job);
-          else
-            job.more = found && round == 0;
+        if (lane == 0) {
+          job.more = more;
           Bars* b = bars;
-          if (!(ok = ptx::mbar_wait(&b->job_empty[round & 1], ((round >> 1) & 1) ^ 1, err))) break;
-          b->job[round & 1] = job;
-          ptx::mbar_arrive(&b->job_full[round & 1]);
-          if (!job.more) break;
+          if ((ok = ptx::mbar_wait(&b->job_empty[round & 1], ((round >> 1) & 1) ^ 1, err))) {
+            b->job[round & 1] = job;
+            ptx::mbar_arrive(&b->job_full[round & 1]);
+          }
+        }
+        if (lane == 0 && ok && more) {
           const Item& it = job.it;
           const int hk = job.hk;
           const int n0 = tile_count(p, it, 0), n1 = tile_count(p, it, 1), n = max(n0, n1);
@@ -622,17 +711,21 @@ __global__ void __launch_bounds__(kThreads, 1)
               phase ^= 1;
             }
           };
-          if (n == 0) continue;
-          if (n0 > 0) load_q(0);
-          load_kv(&tm_k, 0);
-          if (n1 > 0) load_q(1);
-          const int ahead = shared_item(p, it) ? 2 : S::kAhead;
-          if (ahead == 2 && n > 1) load_kv(&tm_k, 1);
-          for (int j = 0; j < n && ok; ++j) {
-            load_kv(&tm_v, j);
-            if (j + ahead < n) load_kv(&tm_k, j + ahead);
+          if (n > 0) {
+            if (n0 > 0) load_q(0);
+            load_kv(&tm_k, 0);
+            if (n1 > 0) load_q(1);
+            const int ahead = shared_item(p, it) ? 2 : S::kAhead;
+            if (ahead == 2 && n > 1) load_kv(&tm_k, 1);
+            for (int j = 0; j < n && ok; ++j) {
+              load_kv(&tm_v, j);
+              if (j + ahead < n) load_kv(&tm_k, j + ahead);
+            }
           }
         }
+        if (!__shfl_sync(0xffffffffu, int(ok && more), 0)) break;
+      }
+      if (lane == 0) {
         // the loads in flight land before the CTA can exit (bounded)
         auto landed = [&](uint64_t* bar, uint32_t parity) {
           const unsigned long long t0 = ptx::globaltimer();
@@ -1204,15 +1297,14 @@ gdc_status launch_typed(const PackedAttentionArgs& a, cudaStream_t stream, int* 
                                                    S::kSmemBytes);
   }));
   if (ce != cudaSuccess) return set_error(GDC_ERR_CUDA, "packed attention smem attribute: %s", cudaGetErrorString(ce));
-  if (!l.planned) {
-    GDC_CUDA_TRY(launch_overlapped(packed_attention_kernel<T, D, false>, unsigned(l.items_ub * a.kv_heads), kThreads, S::kSmemBytes, 1,
-                                   stream, tq, tk, tv, p));
-    return GDC_OK;
+  const int64_t jobs = (l.planned || l.split ? l.chunks_cap : l.items_ub) * a.kv_heads;
+  const unsigned grid = unsigned(l.planned || l.split ? std::min<int64_t>(sms, jobs) : jobs);
+  if (l.planned) {
+    GDC_CUDA_TRY(launch_overlapped(plan_kernel, 1, kPlanThreads, 0, 1, stream, p));
+    GDC_CUDA_TRY(launch_overlapped(packed_attention_kernel<T, D, true>, grid, kThreads, S::kSmemBytes, 1, stream, tq, tk, tv, p));
+  } else {
+    GDC_CUDA_TRY(launch_overlapped(packed_attention_kernel<T, D, false>, grid, kThreads, S::kSmemBytes, 1, stream, tq, tk, tv, p));
   }
-  GDC_CUDA_TRY(launch_overlapped(plan_kernel, 1, kPlanThreads, 0, 1, stream, p));
-  const int64_t jobs = int64_t(l.chunks_cap) * a.kv_heads;
-  GDC_CUDA_TRY(launch_overlapped(packed_attention_kernel<T, D, true>, unsigned(std::min<int64_t>(sms, jobs)), kThreads, S::kSmemBytes, 1,
-                                 stream, tq, tk, tv, p));
   if (l.split) {
     const int64_t rows = l.items_ub * a.kv_heads * l.rows_cap;
     GDC_CUDA_TRY(launch_overlapped(combine_kernel<T, D>, unsigned(std::min<int64_t>(4 * sms, (rows + 7) / 8)), 256, 0, 1, stream, p));

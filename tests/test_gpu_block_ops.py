@@ -382,6 +382,37 @@ def test_attention_many_sequences(batch, most):
     _attention_case(15, "fp16", lq.tolist(), lk.tolist(), 4, 2, 64, True)
 
 
+@pytest.mark.parametrize("batch,longest,empty", [(1, 300, 0), (33, 1500, 3), (64, 300, 0), (128, 130, 70), (129, 130, 80)])
+@pytest.mark.parametrize("dtype,dim", [("fp16", 64), ("bf16", 128)])
+def test_attention_tokens_of_up_to_many_sequences(batch, longest, empty, dtype, dim):
+    """Single tokens of batches around the sizes at which the calls are planned in another way, some without a query."""
+    rng = np.random.Generator(np.random.PCG64(batch))
+    lk = rng.integers(1, longest, batch)
+    lk[0] = longest * 4
+    lq = np.ones(batch, dtype=int)
+    lq[rng.permutation(batch)[:empty]] = 0
+    _attention_case(30, dtype, lq.tolist(), lk.tolist(), 8, 2, dim, True, first=0 if empty == 0 else 1, behind=0 if empty == 0 else 2)
+
+
+def test_attention_tokens_with_bad_offsets():
+    """Few single tokens: a sequence of bad offsets is skipped and reported, the others are computed."""
+    heads, kv_heads, dim = 8, 2, 64
+    q, k, v = (_normal(31 + i, r, w * dim) for i, (r, w) in enumerate([(6, heads), (4000, kv_heads), (4000, kv_heads)]))
+    qo = torch.arange(7, dtype=torch.int32, device="cuda")
+    ko = torch.tensor([0, 1000, 900, 1500, 3000, 4100, 4000], dtype=torch.int32, device="cuda")
+    got = attention(q, k, v, qo, ko, heads, kv_heads, True)
+    torch.cuda.synchronize()
+    assert _lib().gdc_kernels_check_errors() == 3
+    for b in range(6):
+        if b in (1, 4, 5):
+            assert (got[b] == 7.0).all()
+            continue
+        one = slice(ko[b].item(), ko[b + 1].item())
+        want, tol = attention_definition(q[b:b + 1], k[one], v[one], _offsets([1]), _offsets([one.stop - one.start]), heads, kv_heads,
+                                         True, 0.125, torch.full_like(got[b:b + 1], 7.0))
+        _within(got[b:b + 1], want, tol)
+
+
 def test_attention_refused_overlap_writes_nothing_out_of_place():
     """Offsets that decrease and make later sequences overlap earlier ones: reported, rows outside every sequence
     stay as they were."""
