@@ -95,7 +95,7 @@ struct SplitItem {  // an item whose key range was split: slots [slot, slot + n)
   int q_row, lq, k_row, lk, pos, slot, n, pad;
 };
 struct PlanHeader {
-  int n_items, n_splits;
+  int n_items, n_splits, split_rows;  // split_rows: rows of the largest split item
 };
 
 // Workspace: header, items, split items, partial rows (fp32 O, then reference and sum).
@@ -286,7 +286,8 @@ __device__ void store_row_by_definition(const Params& p, int q_row, int lq, int 
 // short that its partial rows (which cost as much as `over` tiles) weigh much. Two sequences
 // of 256 rows after 6000 keys: 103 us in chunks of four tiles, 77 to 86 us so; a prompt of 4096 tokens
 // in 16 heads of 128: 99 us split, joining not counted, 74 us whole; prompts of 6000, 700 and 300 in 16
-// heads of 64: 157 us split, 123 us whole.
+// heads of 64: 157 us split, 123 us whole; 16 tokens over 700 to 2500 keys of 8 heads: 42 us in chunks of
+// four tiles, 31 us whole.
 template <typename I>
 __device__ __forceinline__ int chunk_length(const Params& p, I head_work, int items, int longest) {
   constexpr I kSms = kPlanSms, kWhole = 1 << 30;
@@ -298,8 +299,8 @@ __device__ __forceinline__ int chunk_length(const Params& p, I head_work, int it
   if (jobs <= kSms / 2) {
     const I one = max(2 + 2 * over, ceil_div(work, kSms - jobs));
     if (one <= 8 + 8 * over) c = one;
-  } else if (over > 0 && I(longest) * kSms <= work + work / 4) {
-    c = kWhole;  // the items even out by themselves
+  } else if ((over > 0 && I(longest) * kSms <= work + work / 4) || (jobs <= kSms && I(longest) * kSms <= 2 * work)) {
+    c = kWhole;  // the items even out by themselves, or fill a round whose longest item is near the mean
   }
   const I room = I(p.chunks_cap) * p.kv_heads - jobs;
   return int(min(kWhole, max(c, ceil_div(work, max(I(1), room)))));
@@ -313,13 +314,13 @@ constexpr int kBuckets = 512;
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(Params p) {
   __shared__ int hist[kBuckets];
   __shared__ unsigned long long s_work;
-  __shared__ int s_items, s_max, s_slots, s_splits;
+  __shared__ int s_items, s_max, s_slots, s_splits, s_rows;
   ptx::grid_launch_next();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = kPlanThreads / 32;
   const int per_item = 2 * p.tile_pos;
   if (threadIdx.x == 0) {
     s_work = 0;
-    s_items = s_max = s_slots = s_splits = 0;
+    s_items = s_max = s_slots = s_splits = s_rows = 0;
   }
   for (int i = threadIdx.x; i < kBuckets; i += kPlanThreads) hist[i] = 0;
   ptx::grid_wait();
@@ -374,7 +375,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(Params p) {
   // More items than the query rows can hold: sequences overlap, so that some offset decreases, which has been
   // reported; nothing is computed.
   if (s_items > p.items_ub) {
-    if (threadIdx.x == 0) *p.header = PlanHeader{0, 0};
+    if (threadIdx.x == 0) *p.header = PlanHeader{0, 0, 0};
     return;
   }
   for (int pass = 0; pass < 2; ++pass) {
@@ -384,6 +385,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(Params p) {
       int slot = -1;
       if (pass == 1 && parts > 1) {
         slot = atomicAdd(&s_slots, parts);
+        atomicMax(&s_rows, min(per_item, lq - pos) * p.group);
         p.splits[atomicAdd(&s_splits, 1)] = SplitItem{q0, lq, k0, lk, pos, slot, parts, 0};
       }
       for (int c = 0; c < parts; ++c) {
@@ -414,6 +416,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(Params p) {
   if (threadIdx.x == 0) {
     p.header->n_items = hist[kBuckets - 1];
     p.header->n_splits = s_splits;
+    p.header->split_rows = s_rows;
   }
 }
 
@@ -551,7 +554,7 @@ __device__ __forceinline__ int plan_in_place(const Params& p) {
   const bool none = items == 0 || items > p.items_ub;  // (overlapping sequences, as in plan_kernel)
   const int chunk = none ? 0 : chunk_length<int>(p, work, items, longest);
   if (blockIdx.x == 0) {
-    int splits = 0, slots = 0;
+    int splits = 0, slots = 0, rows = 0;
     for (int b0 = 0; !none && b0 < p.batch; b0 += 32) {
       const int t = only_item(p, b0 + lane, false, q0, lq, k0, lk);
       const int parts = t > chunk ? (t + chunk - 1) / chunk : 0;
@@ -559,10 +562,12 @@ __device__ __forceinline__ int plan_in_place(const Params& p) {
       const int incl = warp_prefix(parts);
       if (parts > 0)
         p.splits[splits + __popc(split & ((1u << lane) - 1))] = SplitItem{q0, lq, k0, lk, 0, slots + incl - parts, parts, 0};
+      if (parts > 0) rows = max(rows, lq * p.group);
       splits += __popc(split);
       slots += __shfl_sync(0xffffffffu, incl, 31);
     }
-    if (lane == 0) *p.header = PlanHeader{0, splits};
+    rows = __reduce_max_sync(0xffffffffu, rows);
+    if (lane == 0) *p.header = PlanHeader{0, splits, rows};
   }
   return chunk;
 }
@@ -1158,13 +1163,12 @@ __global__ void __launch_bounds__(256) combine_kernel(const Params p) {
   constexpr int PER = D / 32;
   ptx::grid_wait();
   const int lane = threadIdx.x & 31;
-  const int rows_per_item = 2 * p.tile_pos * p.group;
-  const long long total = (long long)p.header->n_splits * p.kv_heads * p.rows_cap;
+  const int rows = p.header->split_rows;  // (few where single tokens of long sequences are split, whatever rows_cap)
+  const long long total = (long long)p.header->n_splits * p.kv_heads * rows;
   for (long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); w < total; w += (long long)gridDim.x * 8) {
-    const int row = int(w % p.rows_cap);
-    const int hk = int(w / p.rows_cap % p.kv_heads);
-    const SplitItem it = p.splits[w / p.rows_cap / p.kv_heads];
-    if (row >= rows_per_item) continue;
+    const int row = int(w % rows);
+    const int hk = int(w / rows % p.kv_heads);
+    const SplitItem it = p.splits[w / rows / p.kv_heads];
     const int pos = it.pos + row / p.group, head = hk * p.group + row % p.group;
     if (pos >= it.lq) continue;
     // 32 splits at a time: a lane has one's reference and sum, every lane its columns of all of them
