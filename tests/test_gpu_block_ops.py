@@ -394,6 +394,13 @@ def test_attention_tokens_of_up_to_many_sequences(batch, longest, empty, dtype, 
     _attention_case(30, dtype, lq.tolist(), lk.tolist(), 8, 2, dim, True, first=0 if empty == 0 else 1, behind=0 if empty == 0 else 2)
 
 
+@pytest.mark.parametrize("dtype,dim", [("fp16", 64), ("bf16", 128)])
+@pytest.mark.parametrize("lk", [[130 + 97 * i for i in range(24)], [20] * 11 + [4000], [700] * 32, [1] * 20, [0] * 10 + [513] * 9])
+def test_attention_tokens_of_many_key_heads(dtype, dim, lk):
+    """Items of more than a round, or of uneven length: split ranges of every length, joined."""
+    _attention_case(33, dtype, [1] * len(lk), lk, 16, 8, dim, True, behind=1)
+
+
 def test_attention_tokens_with_bad_offsets():
     """Few single tokens: a sequence of bad offsets is skipped and reported, the others are computed."""
     heads, kv_heads, dim = 8, 2, 64
