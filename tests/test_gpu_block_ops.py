@@ -401,6 +401,32 @@ def test_attention_tokens_of_many_key_heads(dtype, dim, lk):
     _attention_case(33, dtype, [1] * len(lk), lk, 16, 8, dim, True, behind=1)
 
 
+@pytest.mark.parametrize("dim,batch", [(64, 5), (128, 14), (64, 40)])
+def test_attention_tokens_replayed_with_new_lengths(dim, batch):
+    """A captured call follows the lengths that the offsets hold when it is replayed, whatever it split before."""
+    heads, kv_heads, rows = 16, 8, 9000
+    q, k, v = (_normal(34 + i, r, w * dim) for i, (r, w) in enumerate([(batch, heads), (rows, kv_heads), (rows, kv_heads)]))
+    rng = np.random.Generator(np.random.PCG64(dim + batch))
+    cuts = [np.sort(rng.integers(0, rows, batch - 1)) for _ in range(3)]
+    cuts.append(np.arange(1, batch))  # one sequence has nearly all the keys
+    offs = [torch.tensor(np.concatenate([[0], c, [rows]]), dtype=torch.int32, device="cuda") for c in cuts]
+    qo, ko = torch.arange(batch + 1, dtype=torch.int32, device="cuda"), offs[0].clone()
+    ws, out = _workspace(batch, batch, rows, heads, kv_heads, dim), torch.empty_like(q)
+    attention(q, k, v, qo, ko, heads, kv_heads, True, out=out, ws=ws)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        attention(q, k, v, qo, ko, heads, kv_heads, True, out=out, ws=ws)
+    for off in offs + offs[:1]:
+        ko.copy_(off)
+        out.fill_(7.0)
+        g.replay()
+        _done()
+        sc = np.float32(1 / math.sqrt(dim)).item()
+        want, tol = attention_definition(q, k, v, qo, off, heads, kv_heads, True, sc, torch.full_like(out, 7.0))
+        _within(out, want, tol)
+
+
 def test_attention_tokens_with_bad_offsets():
     """Few single tokens: a sequence of bad offsets is skipped and reported, the others are computed."""
     heads, kv_heads, dim = 8, 2, 64
