@@ -313,26 +313,34 @@ constexpr int kBuckets = 512;
 // where a sequence has many items the lanes share them out.
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(Params p) {
   __shared__ int hist[kBuckets];
-  __shared__ unsigned long long s_work;
-  __shared__ int s_items, s_max, s_slots, s_splits, s_rows;
+  __shared__ unsigned long long s_work, s_items;
+  __shared__ int s_max, s_slots, s_splits, s_rows;
   ptx::grid_launch_next();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = kPlanThreads / 32;
   const int per_item = 2 * p.tile_pos;
   if (threadIdx.x == 0) {
-    s_work = 0;
-    s_items = s_max = s_slots = s_splits = s_rows = 0;
+    s_work = s_items = 0;
+    s_max = s_slots = s_splits = s_rows = 0;
   }
   for (int i = threadIdx.x; i < kBuckets; i += kPlanThreads) hist[i] = 0;
   ptx::grid_wait();
   __syncthreads();
   const int run = (p.batch + warps - 1) / warps;  // sequences of a warp
-  // f(q0, lq, k0, lk, position, key tiles) for every item; a sequence of bad offsets has none
-  auto for_each_item = [&](bool report, auto&& f) {
+  // f(q0, lq, k0, lk, position, key tiles) for every item; a sequence of bad offsets has none. The first pass
+  // reports those and counts the warp's items, in 64 bits: offsets that decrease can make 2^19 sequences
+  // overlap, each of them as long as the query rows. A warp that has counted more than the rows can hold
+  // goes over no more items (nothing will be computed), so that the passes end whatever the offsets are.
+  auto for_each_item = [&](bool first, auto&& f) {
     const int last = min(p.batch, (warp + 1) * run);
+    long long count = 0;
     for (int b0 = warp * run; b0 < last; b0 += 32) {
       int q0 = 0, lq = 0, k0 = 0, lk = 0;
-      if (b0 + lane < last && !sequence(p, b0 + lane, report, q0, lq, k0, lk)) lq = 0;
-      const int n = (lq + per_item - 1) / per_item;
+      if (b0 + lane < last && !sequence(p, b0 + lane, first, q0, lq, k0, lk)) lq = 0;
+      const int n = (lq + per_item - 1) / per_item;  // (below 2^30)
+      if (first) {
+        count += __reduce_add_sync(0xffffffffu, n & 0xffff) + ((long long)__reduce_add_sync(0xffffffffu, n >> 16) << 16);
+        if (count > p.items_ub) continue;
+      }
       auto item = [&](int q, int l, int k, int m, int i) {
         const int pos = i * per_item;
         f(q, l, k, m, pos, (seen_keys(min(pos + per_item, l) - 1, l, m, p.causal) + kKeys - 1) / kKeys);
@@ -348,36 +356,35 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(Params p) {
       }
     }
     __syncwarp();
+    return count;
   };
   {
     unsigned long long work = 0;
-    int items = 0, most = 0;
-    for_each_item(true, [&](int, int, int, int, int, int t) {
+    int most = 0;
+    const long long items = for_each_item(true, [&](int, int, int, int, int, int t) {
       work += t;
-      ++items;
       most = max(most, t);
     });
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) work += __shfl_xor_sync(0xffffffffu, work, o);
-    items = __reduce_add_sync(0xffffffffu, items);
     most = __reduce_max_sync(0xffffffffu, most);
     if (lane == 0) {
       atomicAdd(&s_work, work);
-      atomicAdd(&s_items, items);
+      atomicAdd(&s_items, (unsigned long long)items);
       atomicMax(&s_max, most);
     }
   }
   __syncthreads();
-  const int chunk = p.can_split ? chunk_length<long long>(p, (long long)s_work, s_items, s_max) : 1 << 30;
-  int shift = 0;
-  while ((min(chunk, s_max) >> shift) >= kBuckets) ++shift;
-  auto bucket = [&](int tiles) { return kBuckets - 1 - min(kBuckets - 1, tiles >> shift); };
   // More items than the query rows can hold: sequences overlap, so that some offset decreases, which has been
-  // reported; nothing is computed.
-  if (s_items > p.items_ub) {
+  // reported; nothing is computed. (This is what keeps the lists below inside the workspace.)
+  if (s_items > (unsigned long long)p.items_ub) {
     if (threadIdx.x == 0) *p.header = PlanHeader{0, 0, 0};
     return;
   }
+  const int chunk = p.can_split ? chunk_length<long long>(p, (long long)s_work, int(s_items), s_max) : 1 << 30;
+  int shift = 0;
+  while ((min(chunk, s_max) >> shift) >= kBuckets) ++shift;
+  auto bucket = [&](int tiles) { return kBuckets - 1 - min(kBuckets - 1, tiles >> shift); };
   for (int pass = 0; pass < 2; ++pass) {
     for_each_item(false, [&](int q0, int lq, int k0, int lk, int pos, int t) {
       const int parts = t > chunk ? (t + chunk - 1) / chunk : 1;

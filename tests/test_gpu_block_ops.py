@@ -458,6 +458,21 @@ def test_attention_refused_overlap_writes_nothing_out_of_place():
     assert (got[n:] == 7.0).all()
 
 
+@pytest.mark.parametrize("heads,rows", [(1, 1 << 20), (128, 1 << 17)])
+def test_attention_refuses_overlaps_whose_items_pass_32_bits(heads, rows):
+    """Offsets 0, rows, 0, rows, ...: every other sequence overlaps all the others, 2^31 and 2^32 items in all (256
+    and 2 query rows each). Reported, and nothing is computed."""
+    per_item = 2 * (128 // heads)
+    assert rows // 2 * (rows // per_item) == (1 << 31 if heads == 1 else 1 << 32)
+    q, kv = torch.zeros(rows, heads * 64, dtype=torch.float16, device="cuda"), _normal(19, 64, 64)
+    odd = torch.arange(rows + 1, dtype=torch.int32, device="cuda") % 2
+    got = attention(q, kv, kv, odd * rows, odd * 64, heads, 1, True)
+    torch.cuda.synchronize()
+    assert _lib().gdc_kernels_check_errors() == 3
+    assert (got == 7.0).all()
+    _done()
+
+
 def test_attention_shared_workspace_in_turn():
     """Two captured calls on one workspace, replayed one after the other, again and again."""
     dim, heads = 64, 4
