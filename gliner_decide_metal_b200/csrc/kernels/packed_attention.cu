@@ -26,8 +26,10 @@
 // its key tiles in turn (shared_item).
 //
 // The reference m_i moves only when a row's maximum has grown by more than 2^8 (then the tile's
-// O rows are rescaled in TMEM): weights stay below 2^8, which 16-bit weights and fp32 sums hold
-// without loss, and most key tiles need no rescale. S_t(j) complete implies P_t V(j-1) complete
+// O rows are rescaled in TMEM), so most key tiles need no rescale. The weights are rounded to the tensors'
+// type: bf16 has fp32's range; in fp16 they are computed 2^7 larger (the factor is in O and in the row's sum
+// alike), so they reach up to 2^15, the range's end, and its lower end is that much further away: a weight
+// is off by 2^-11 of itself or by 2^-32 of the largest one, whichever is more. S_t(j) complete implies P_t V(j-1) complete
 // (one thread issues them in that order) at D = 128, so the rescale needs no wait of its own; at D = 64
 // the row warps wait for P_t V(j-1) before they write O_t or P_t. The weights are
 // rounded to the tensors' type for the second product, the row's sum is of the unrounded ones.
@@ -78,6 +80,7 @@ constexpr int kRowRegs = 216, kIssueRegs = 72;  // 256 * 216 + 128 * 72 = 384 * 
 constexpr int kPlanThreads = 512;
 constexpr int kPlanSms = 148;    // the planner's unit of work (the workspace size depends on it)
 constexpr float kGrowth = 8.0f;  // log2 growth of a row's maximum that moves its reference
+constexpr float kHalfLift = 7.0f;  // log2 of the factor of fp16 weights
 
 // One work item (32 bytes).
 struct Item {
@@ -966,6 +969,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int row_pos = r / p.group, row_head = r % p.group;
     const int warp_pos = ((warp & 3) * 32) / p.group;
     const float c = p.scale_log2;
+    constexpr float kLift = E::kMmaFormat == 0 ? kHalfLift : 0.f;
     uint32_t s_uses = 0, o_uses = 0, joins = 0;
     float2* ml = reinterpret_cast<float2*>(smem + S::kOffMl) + r;
     bool ok = true;
@@ -1025,7 +1029,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float top = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], m);
         if (j == 0) {
           m = top;
-          mc = m == -INFINITY ? 0.f : m * c;
+          mc = m == -INFINITY ? 0.f : fmaf(m, c, -kLift);
         } else {
           if (S::kOwnP) {  // the last product has read the weights and written O
             ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->o_full[t], o_uses & 1, err));
@@ -1038,7 +1042,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float f = grow ? ex2(m * c - top * c) : 1.f;
             if (grow) {
               m = top;
-              mc = m * c;
+              mc = fmaf(m, c, -kLift);
             }
             sum0.x *= f;
             sum0.y *= f;

@@ -197,6 +197,25 @@ def test_attention_growing_scores():
 
 
 @pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("rows,n", [(1, 250), (1, 6000), (150, 2000)])
+@pytest.mark.parametrize("gap", [8.0, 14.0, 17.0, 17.375, 20.0])
+def test_attention_small_weights_beside_a_dominant_key_of_zeros(dim, rows, n, gap):
+    """One key outweighs every other by e^gap and its value row is zero, so the small weights are all there is. fp16
+    weights have 2^-11 of themselves, or 2^-32 of the largest one (half the smallest fp16 step, 2^-25, at
+    weights that are computed 2^7 larger)."""
+    q, k, v = torch.zeros(rows, dim).half().cuda(), torch.zeros(n, dim).half().cuda(), 32 + 32 * _normal(37, n, dim).abs().clamp(max=1)
+    q[:, 0], k[0, 0], v[0] = 1.0, gap, 0.0
+    got = attention(q, k, v, _offsets([rows]), _offsets([n]), 1, 1, False, 1.0)
+    _done()
+    s = q.double() @ k.double().t()
+    w = torch.softmax(s, -1)
+    want = w @ v.double()
+    u, ds = 2.0 ** -11, (dim + 8) * 2.0 ** -23 * gap
+    tol = 2.0 ** -32 * w.amax(1, keepdim=True) * v.double().sum(0) + 2 * (u + 2.0 ** -22 + n * 2.0 ** -23 + 2 * ds) * want + u * want
+    _within(got, want, tol)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("rows", [1, 3, 200])
 def test_attention_growing_scores_of_a_sequences_last_rows(dim, rows):
     """The same where one query tile's key tiles are taken in turn by both row groups, and in split ranges."""
