@@ -81,6 +81,10 @@ constexpr int kPlanThreads = 512;
 constexpr int kPlanSms = 148;    // the planner's unit of work (the workspace size depends on it)
 constexpr float kGrowth = 8.0f;  // log2 growth of a row's maximum that moves its reference
 constexpr float kHalfLift = 7.0f;  // log2 of the factor of fp16 weights
+// A row's reference in log2 units is rounded to fp32. Beyond this (scores of 2.9 million) the rounding would
+// move its weights by more than a quarter of a binade, and further out past what 16 bits hold: such a
+// row is computed by its definition (row_by_definition), from differences of scores.
+constexpr float kMaxReference = 4194304.f;
 
 // One work item (32 bytes).
 struct Item {
@@ -1084,6 +1088,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) break;
       // ---- the item's rows of this tile
       float l = (sum0.x + sum0.y) + (sum1.x + sum1.y);
+      if (fabsf(mc) > kMaxReference) l = NAN;  // (in a split's or group's partial row: of the joined row)
       const Item it = job->it;
       const int hk = job->hk;
       const int head = hk * p.group + row_head, pos = it.pos + t * p.tile_pos + row_pos;

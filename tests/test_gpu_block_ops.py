@@ -215,6 +215,24 @@ def test_attention_small_weights_beside_a_dominant_key_of_zeros(dim, rows, n, ga
     _within(got, want, tol)
 
 
+@pytest.mark.parametrize("dtype,dim", [("fp16", 64), ("fp16", 128), ("bf16", 64), ("bf16", 128)])
+@pytest.mark.parametrize("rows,n", [(1, 1), (1, 6000), (150, 400)])
+@pytest.mark.parametrize("scale", [0.125, 0.875, 1.0])
+def test_attention_scores_beyond_what_fp32_counts_in(dtype, dim, rows, n, scale):
+    """Scores of 10^6 to 10^11 whose largest is one key's by far: the output is that key's value row. The reference in log2
+    units is rounded by up to a quarter, so the key's weight, 2^that, need not be a power of two: it is off by
+    u when it is rounded to 16 bits (the row's sum takes it unrounded), and the output once more by u."""
+    t = DTYPES[dtype][0]
+    v = _normal(38, n, dim, dtype=t)
+    for size in (400.0, 1000.0, 10000.0, 20000.0, 30000.0):
+        q, k = torch.full((rows, dim), size, dtype=t, device="cuda"), torch.full((n, dim), size / 2, dtype=t, device="cuda")
+        k[n // 2] = size
+        got = attention(q, k, v, _offsets([rows]), _offsets([n]), 1, 1, False, scale)
+        _done()
+        want = v[n // 2].double().expand(rows, dim)
+        _within(got, want, 2.02 * torch.finfo(t).eps / 2 * want.abs())
+
+
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("rows", [1, 3, 200])
 def test_attention_growing_scores_of_a_sequences_last_rows(dim, rows):
