@@ -162,6 +162,7 @@ struct Params {
   long long items_ub;
   int wide_out;  // out's rows are 32-byte aligned
   int can_split;
+  unsigned long long wait_ns;  // limit of the waits that rows computed by their definition can hold up (not of those for loads)
   int* err;
 };
 
@@ -646,8 +647,8 @@ struct Jobs {
   Bars* bars;
   uint32_t n = 0;
   // Waits for the next job (all lanes of a warp); null: no more, or a wait gave up.
-  __device__ __forceinline__ const Job* next(int* err) {
-    if (!__all_sync(0xffffffffu, ptx::mbar_wait(&bars->job_full[n & 1], (n >> 1) & 1, err))) return nullptr;
+  __device__ __forceinline__ const Job* next(int* err, unsigned long long wait_ns) {
+    if (!__all_sync(0xffffffffu, ptx::mbar_wait(&bars->job_full[n & 1], (n >> 1) & 1, err, wait_ns))) return nullptr;
     const Job* job = &bars->job[n & 1];
     return job->more ? job : nullptr;
   }
@@ -728,7 +729,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) {
           job.more = more;
           Bars* b = bars;
-          if ((ok = ptx::mbar_wait(&b->job_empty[round & 1], ((round >> 1) & 1) ^ 1, err))) {
+          if ((ok = ptx::mbar_wait(&b->job_empty[round & 1], ((round >> 1) & 1) ^ 1, err, p.wait_ns))) {
             b->job[round & 1] = job;
             ptx::mbar_arrive(&b->job_full[round & 1]);
           }
@@ -738,7 +739,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int hk = job.hk;
           const int n0 = tile_count(p, it, 0), n1 = tile_count(p, it, 1), n = max(n0, n1);
           auto load_q = [&](int t) {
-            if (!(ok = ok && ptx::mbar_wait(&bars->q_empty[t], (q_uses[t] & 1) ^ 1, err))) return;
+            if (!(ok = ok && ptx::mbar_wait(&bars->q_empty[t], (q_uses[t] & 1) ^ 1, err, p.wait_ns))) return;
             ++q_uses[t];
             ptx::mbar_arrive_expect_tx(&bars->q_full[t], uint32_t(S::kAtoms * p.tile_pos * p.group * 128));
             for (int a = 0; a < S::kAtoms; ++a)
@@ -746,7 +747,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                it.q_row + it.pos + t * p.tile_pos, &bars->q_full[t]);
           };
           auto load_kv = [&](const CUtensorMap* map, int j) {
-            if (!(ok = ok && ptx::mbar_wait(&bars->empty[stage], phase ^ 1, err))) return;
+            if (!(ok = ok && ptx::mbar_wait(&bars->empty[stage], phase ^ 1, err, p.wait_ns))) return;
             ptx::mbar_arrive_expect_tx(&bars->full[stage], uint32_t(S::kTileBytes));
             for (int a = 0; a < S::kAtoms; ++a)
               ptx::tma_load_2d(s_ring + stage * S::kTileBytes + a * 16384, map, hk * D + a * 64,
@@ -795,7 +796,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t q1_skipped = 0;  // shared items: group 1 took part without a query tile of its own
       bool ok = true;
       while (ok) {
-        const Job* job = jobs.next(err);
+        const Job* job = jobs.next(err, p.wait_ns);
         if (job == nullptr) break;
         const int cnt[2] = {tile_count(p, job->it, 0), tile_count(p, job->it, 1)};
         const int n = max(cnt[0], cnt[1]);
@@ -845,7 +846,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         };
         // the weights of P_t, and before its first product of an item, O_t's columns
         auto weights_ready = [&](int t, bool first) {
-          bool got = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->p_ready[t], p_uses[t] & 1, err));
+          bool got = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->p_ready[t], p_uses[t] & 1, err, p.wait_ns));
           ++p_uses[t];
           if (got && first) got = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->o_free[t], (items_of[t] & 1) ^ 1, err));
           ptx::tc_fence_after();
@@ -903,7 +904,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         advance();
         // S_t's columns have been read (step p_uses[t] of this tile, counted over the items)
         auto scores_read = [&](int t) {
-          const bool got = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->s_free[t], p_uses[t] & 1, err));
+          const bool got = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->s_free[t], p_uses[t] & 1, err, p.wait_ns));
           ptx::tc_fence_after();
           return got;
         };
@@ -978,7 +979,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     float2* ml = reinterpret_cast<float2*>(smem + S::kOffMl) + r;
     bool ok = true;
     while (true) {
-      const Job* job = jobs.next(err);
+      const Job* job = jobs.next(err, p.wait_ns);
       if (job == nullptr) break;
       // key tiles of this group; keys that the row, and the warp's first row, see from the range's first on;
       // keys from one of the group's tiles to the next
@@ -1001,7 +1002,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       float m = -INFINITY, mc = 0.f;
       float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
       for (int j = 0; j < n; ++j) {
-        ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->s_full[t], s_uses & 1, err));
+        ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->s_full[t], s_uses & 1, err, p.wait_ns));
         ++s_uses;
         if (!ok) break;
         ptx::tc_fence_after();
@@ -1036,7 +1037,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           mc = m == -INFINITY ? 0.f : fmaf(m, c, -kLift);
         } else {
           if (S::kOwnP) {  // the last product has read the weights and written O
-            ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->o_full[t], o_uses & 1, err));
+            ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->o_full[t], o_uses & 1, err, p.wait_ns));
             ++o_uses;
             if (!ok) break;
             ptx::tc_fence_after();
@@ -1101,7 +1102,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // factors of O_t and, in a shared item, of group 1's O
       float f0 = !scaled ? 1.f : seen > 0 ? 1.f / l : 0.f, f1 = 0.f;
       if (n > 0) {
-        ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->o_full[t], o_uses & 1, err));
+        ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->o_full[t], o_uses & 1, err, p.wait_ns));
         ++o_uses;
         if (!ok) break;
         ptx::tc_fence_after();
@@ -1116,7 +1117,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         continue;
       }
       if (shared) {
-        ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->ml_ready, joins & 1, err));  // O_1 is complete too
+        ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->ml_ready, joins & 1, err, p.wait_ns));  // O_1 is complete too
         if (!ok) break;
         ptx::tc_fence_after();
         ++joins;
@@ -1333,6 +1334,9 @@ gdc_status launch_typed(const PackedAttentionArgs& a, cudaStream_t stream, int* 
   p.chunks_cap = l.chunks_cap;
   p.items_ub = l.items_ub;
   p.can_split = l.split;
+  // A warp may have 32 rows to compute by their definition, 130 to 190 ns a key each, while others wait for it, and a
+  // wait may see two such warps one after the other: 2 s would be over with 180,000 keys. A microsecond a key and row.
+  p.wait_ns = ptx::kTimeoutNs + 64 * 1000ull * (unsigned long long)a.k_rows;
   p.err = err;
   p.wide_out = reinterpret_cast<uintptr_t>(a.out) % 32 == 0 && a.ldo % 16 == 0;
 

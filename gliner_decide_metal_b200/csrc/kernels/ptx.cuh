@@ -72,9 +72,9 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 constexpr unsigned long long kErrCheckNs = 1000000ull;  // 1 ms
 
 // Waits until the phase with `parity` has completed. Returns false (and flags
-// kErrTimeoutBit in *err) if it does not within kTimeoutNs, or if another thread
+// kErrTimeoutBit in *err) if it does not within `limit_ns`, or if another thread
 // of the grid has already flagged a timeout (seen after kErrCheckNs of waiting).
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* err) {
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* err, unsigned long long limit_ns = kTimeoutNs) {
   if (mbar_try_wait(bar, parity)) return true;
   const unsigned long long t0 = globaltimer();
   for (uint32_t i = 1;; ++i) {
@@ -83,7 +83,7 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* e
       const unsigned long long dt = globaltimer() - t0;
       if (dt > kErrCheckNs) {
         if (*reinterpret_cast<volatile int*>(err) & kErrTimeoutBit) return false;
-        if (dt > kTimeoutNs) {
+        if (dt > limit_ns) {
           atomicOr(err, kErrTimeoutBit);
           return false;
         }

@@ -301,6 +301,26 @@ def test_attention_keeps_what_is_not_seen_out(dtype, dim, bad):
         assert torch.isnan(got[150:200, :2 * dim]).all()
 
 
+def test_attention_infinite_value_behind_many_keys():
+    """64 rows that see an infinite value among 600,000 keys are computed by their definition, 32 by each of two warps one
+    after the other (about 3 s); the CTA's other warps wait for them and its further items are computed."""
+    dim, n, rows = 64, 600_000, 256 * 1200
+    q, k, v = _normal(39, rows, dim), _normal(40, n, dim), _normal(41, n, dim, std=0.5, mean=1.0)
+    v[n - 64, 0] = math.inf
+    got = attention(q, k, v, _offsets([rows]), _offsets([n]), 1, 1, True, 0.125)
+    _done()
+    assert (got[-64:, 0] == math.inf).all() and torch.isfinite(got[:-64]).all() and torch.isfinite(got[-64:, 1:]).all()
+    at = torch.tensor([0, 1000, 150_000, rows - 300, rows - 65, *range(rows - 64, rows)], device="cuda")
+    v[n - 64, 0] = 0
+    seen = (at + n - rows + 1)[:, None] > torch.arange(n, device="cuda")
+    w = torch.softmax((q[at].double() @ k.double().t() * 0.125).masked_fill(~seen, -math.inf), -1)
+    want, reach = w @ v.double(), w @ v.double().abs()
+    ds = (dim + 8) * 2.0 ** -23 * (q[at].double().abs() @ k.double().abs().t() * 0.125).amax(1, keepdim=True)
+    tol = (2.0 ** -11 + 2.0 ** -22 + n * 2.0 ** -23 + 2 * ds) * (reach + want.abs()) + 2.0 ** -11 * want.abs()
+    _within(got[at][:, 1:], want[:, 1:], tol[:, 1:])
+    assert (got > 0.5).all() and (got[:-64] < 1.5).all()  # (a row that was left out is 7)
+
+
 def test_attention_skips_and_reports_bad_offsets():
     """Offsets that decrease or leave the rows: that sequence is skipped and reported, the others
     are computed."""
