@@ -11,7 +11,8 @@
 // slots of shared memory (cp.async; no other thread reads them, so nothing is synchronised) while
 // it works on this one, and a row belongs to few threads: one warp up to 512
 // columns (reductions without a barrier, four rows a block), one block of 64 to 512 threads above.
-// Weights and gate rows are read again for every row, from L1. Rows at odd 2-byte addresses are read
+// Weights and gate rows are read again for every row, from L1, by plain loads: the kernel may be resident while
+// the one before it writes them, so they are not read-only for its lifetime. Rows at odd 2-byte addresses are read
 // value by value when their turn comes.
 //
 // On a B200, two norms and a gate (8 bytes a value): 16384 x 4096 RMSNorm 90 us, 6.0 TB/s (0.91 of a
@@ -51,17 +52,17 @@ struct Values {
       const int col = first + c * step;
       if (V == 8) {
         uint4 r = make_uint4(0u, 0u, 0u, 0u);
-        if (col < cols) r = STREAM ? __ldcs(reinterpret_cast<const uint4*>(p + col)) : __ldg(reinterpret_cast<const uint4*>(p + col));
+        if (col < cols) r = STREAM ? __ldcs(reinterpret_cast<const uint4*>(p + col)) : *reinterpret_cast<const uint4*>(p + col);
         w[c * 4 % kWords] = r.x;
         w[(c * 4 + 1) % kWords] = r.y;
         w[(c * 4 + 2) % kWords] = r.z;
         w[(c * 4 + 3) % kWords] = r.w;
       } else if (V == 2) {
         const uint32_t* q = reinterpret_cast<const uint32_t*>(p + col);
-        w[c % kWords] = col < cols ? (STREAM ? __ldcs(q) : __ldg(q)) : 0u;
+        w[c % kWords] = col < cols ? (STREAM ? __ldcs(q) : *q) : 0u;
       } else {
         const uint16_t* q = reinterpret_cast<const uint16_t*>(p + col);
-        w[c % kWords] = col < cols ? uint32_t(STREAM ? __ldcs(q) : __ldg(q)) : 0u;
+        w[c % kWords] = col < cols ? uint32_t(STREAM ? __ldcs(q) : *q) : 0u;
       }
     }
   }
@@ -224,7 +225,7 @@ __global__ void __launch_bounds__(NormShape<V, N, TPR>::kThreads, NormShape<V, N
     for (int s = 0; s < kStages - 1; ++s) fetch(row + s * stride, s);
   for (; row < n_rows; row += stride) {  // (uniform over the threads of a row, which share its barriers)
     long long g_row = p.gate_rows == 1 ? 0 : row;
-    if (p.gate_index != nullptr) g_row = __ldg(p.gate_index + row);
+    if (p.gate_index != nullptr) g_row = p.gate_index[row];
     float xv[N], z[N];
     {
       Values<T, V, N> xr, yr;

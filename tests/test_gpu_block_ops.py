@@ -992,6 +992,31 @@ def test_calls_follow_each_other_without_waiting():
     assert torch.isfinite(a).all() and torch.equal(a, b)
 
 
+@pytest.mark.parametrize("cols", [512, 514, 515])
+def test_norm_follows_a_gate_that_the_call_before_it_writes(cols):
+    """Gate rows, weights and indices change between the calls of a chain: the gate and the weight are each written by the
+    linear just before the norm that reads them. Against the same chain with a wait after every call."""
+    def chain(wait):
+        rows, gates = 700, 9
+        x, y = _normal(210, rows, cols), _normal(211, rows, cols)
+        c, w = _normal(212, 40, gates, 64), [_normal(213 + i, cols, 64, std=0.1) for i in range(3)]
+        gate, weight = (torch.zeros(n, cols, dtype=torch.float16, device="cuda") for n in (gates, 1))
+        index = (torch.arange(rows, device="cuda") % gates).int()
+        for i in range(40):
+            linear(c[i], w[i % 3], None, None, 0, out=gate)
+            wait()
+            norm(y, x, "rms", weight[0] if i else None, None, gate, index if i % 3 else index.roll(i), 0.5, "rms", None, None, 1e-6,
+                 x_out=x, n_out=y)
+            wait()
+            linear(c[i][:1], w[(i + 1) % 3], None, None, 0, out=weight)
+            wait()
+        torch.cuda.synchronize()
+        return x
+    a, b = chain(lambda: None), chain(torch.cuda.synchronize)
+    _done()
+    assert torch.isfinite(a).all() and torch.equal(a, b)
+
+
 def test_first_use_of_a_kernel_inside_a_capture():
     """Only the first call on a device has to come before a capture; a kernel first used inside one works."""
     import subprocess
