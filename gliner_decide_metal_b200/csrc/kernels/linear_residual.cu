@@ -83,10 +83,10 @@ __device__ __forceinline__ void tile_at(long long t, int num_n, int num_m, int& 
 }
 
 // The activation of two values (rows m, m + 1 of one n).
-template <int ACT>
+template <typename T, int ACT>
 __device__ __forceinline__ float2 activate(float2 z) {
   if (ACT == kActGelu) {
-    const float2 g = gelu_erf2(z);
+    const float2 g = ElemOps<T>::kMmaFormat == 1 ? gelu_erf2_wide(z) : gelu_erf2(z);
     return make_float2(z.x > 16.f ? z.x : g.x, z.y > 16.f ? z.y : g.y);  // GELU(x) = x there; keeps +inf
   }
   if (ACT == kActRelu) {
@@ -124,7 +124,7 @@ struct Column {
     float v[16];
 #pragma unroll
     for (int i = 0; i < 16; i += 2) {
-      const float2 x = activate<ACT>(__fadd2_rn(make_float2(__uint_as_float(z[i]), __uint_as_float(z[i + 1])), make_float2(bias, bias)));
+      const float2 x = activate<T, ACT>(__fadd2_rn(make_float2(__uint_as_float(z[i]), __uint_as_float(z[i + 1])), make_float2(bias, bias)));
       v[i] = x.x;
       v[i + 1] = x.y;
     }
@@ -396,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!live || m >= M) continue;
         float z = 0.f;
         for (int s = 0; s < p.split; ++s) z += red[(s * mine + j) * 128 + quarter * 32 + lane];
-        z = activate<ACT>(make_float2(z + bias, 0.f)).x;
+        z = activate<T, ACT>(make_float2(z + bias, 0.f)).x;
         if (res != nullptr) z += E::to_f32(res[m * p.ldr + n]);
         out[m * p.ldo + n] = E::from_f32(z);
       }

@@ -663,6 +663,25 @@ def test_linear_carries_infinities_and_nan():
         assert torch.isnan(got[17]).all()
 
 
+@pytest.mark.parametrize("M", [1, 2, 300])
+def test_linear_gelu_of_far_negative_values_in_bf16(M):
+    """bf16 holds GELU(-6) = -6e-9 and GELU(-13) = -8e-38 like any other value: relative to the result, half a step (2^-8) and
+    2^-14 of the evaluation (the fit's 1e-6, an exponent of up to 126 in fp32: 126 * 2^-24 ln 2 = 5e-6 for each of its
+    three roundings). The power of two is zero below 2^-126 and its factor at most 1.2: results below 2^-125 may be zero."""
+    t = torch.bfloat16
+    z = torch.linspace(-14, -4, 1601, device="cuda").to(t)
+    a, w = torch.zeros(M, 8, dtype=t, device="cuda"), torch.zeros(z.numel(), 8, dtype=t, device="cuda")
+    a[:, 0], w[:, 0] = 1.0, z
+    got = linear(a, w, None, None, 1)
+    _done()
+    zd = z.double()
+    want = (0.5 * zd * torch.special.erfc(-zd / math.sqrt(2))).expand(M, -1)
+    for far in (-20.0, -1e10, -3e38):
+        w[:, 0] = far
+        assert (linear(a, w, None, None, 1) == 0).all()
+    _within(got, want, (2.0 ** -8 + 2.0 ** -14) * want.abs() + 2.0 ** -125)
+
+
 def test_linear_captured_and_replayed():
     a, w, x = _normal(76, 90, 512), _normal(77, 520, 512, std=0.05), _normal(78, 90, 520)
     rows = torch.tensor([90], dtype=torch.int32, device="cuda")
