@@ -722,11 +722,28 @@ gdc_status gdc_kernels_check_errors(void) {
   GDC_CUDA_TRY(cudaMemcpy(&h, err, sizeof(int), cudaMemcpyDeviceToHost));
   if (h != 0) {
     GDC_CUDA_TRY(cudaMemset(err, 0, sizeof(int)));
-    if (h & kErrTimeout) return set_error(GDC_ERR_TIMEOUT, "a device-side wait exceeded its time limit");
-    if (h & kErrBadOffsets)
-      return set_error(GDC_ERR_INVALID_INPUT, "packed offsets decrease or leave the buffers' rows");
-    if (h & kErrBadGateIndex) return set_error(GDC_ERR_INVALID_INPUT, "a gate index is outside [0, gate_rows)");
-    return set_error(GDC_ERR_CUDA, "device error word 0x%x", h);
+    // one status (the first of these that is set), and a message that names all that was
+    static const struct {
+      int bit;
+      gdc_status status;
+      const char* what;
+    } known[] = {{kErrTimeout, GDC_ERR_TIMEOUT, "a device-side wait exceeded its time limit"},
+                 {kErrBadOffsets, GDC_ERR_INVALID_INPUT, "packed offsets decrease or leave the buffers' rows"},
+                 {kErrBadGateIndex, GDC_ERR_INVALID_INPUT, "a gate index is outside [0, gate_rows)"}};
+    gdc_status status = GDC_OK;
+    char what[512] = "";
+    size_t at = 0;
+    for (const auto& k : known) {
+      if (!(h & k.bit)) continue;
+      if (status == GDC_OK) status = k.status;
+      at += size_t(snprintf(what + at, sizeof(what) - at, "%s%s", at ? "; " : "", k.what));
+      h &= ~k.bit;
+    }
+    if (h != 0) {
+      if (status == GDC_OK) status = GDC_ERR_CUDA;
+      snprintf(what + at, sizeof(what) - at, "%sdevice error word 0x%x", at ? "; " : "", h);
+    }
+    return set_error(status, "%s", what);
   }
   return GDC_OK;
 }

@@ -333,8 +333,9 @@ gdc_status gdc_linear(const uint16_t* a, const uint16_t* w, const uint16_t* bias
  *    capture. A captured call may be replayed with new contents of every tensor, offsets,
  *    indices and row counts included.
  *  - What only the device can see (offsets, indices) is checked there: a bad value is skipped
- *    as described below, never followed out of range, and the next gdc_kernels_check_errors()
- *    returns GDC_ERR_INVALID_INPUT.
+ *    as described below, never followed out of range, and reported by the next
+ *    gdc_kernels_check_errors() (GDC_ERR_INVALID_INPUT; GDC_ERR_TIMEOUT if a wait ran out too, with
+ *    both in the message).
  *  - rows_dev (may be NULL): a device int32, read when the call runs; only rows
  *    [0, min(rows, *rows_dev)) are computed and written, rows behind them stay as they were. With
  *    packed sequences this is the last entry of the offsets.
@@ -402,7 +403,9 @@ gdc_status gdc_gated_residual_norm(gdc_dtype dtype, const void* y, int64_t ldy, 
                                    const int32_t* rows_dev, int32_t cols, float eps, void* stream);
 
 /* Reads and clears the current device's error word used by the kernel-level entry
- * points above (bounded-wait timeouts, bad offsets and indices). Synchronises the device. */
+ * points above (bounded-wait timeouts, bad offsets and indices). Synchronises the device. The word
+ * is the device's: it holds what any caller's calls have raised since it was last read, and
+ * gdc_last_error() names all of it. */
 gdc_status gdc_kernels_check_errors(void);
 
 /* Failure-detection self-test (no counterpart in the reference): launches a kernel whose

@@ -878,6 +878,30 @@ def test_norm_skips_and_reports_bad_gate_indices():
     _done()
 
 
+def test_errors_of_several_calls_are_all_named():
+    """The error word holds what every call since its last reading has raised: one status, and a message that names all."""
+    lib = _lib()
+    y, x, pw, pb, g, nw, nb = _norm_inputs(96, 12, 256, "rms", "rms", 4, "fp16")
+    q = _normal(32, 8, 64)
+
+    def bad_index():
+        norm(y, x, "rms", pw, None, g, torch.full((12,), 4, dtype=torch.int32, device="cuda"), 1.0, "rms", nw, None, 1e-6)
+
+    def bad_offsets():
+        attention(q, q, q, torch.tensor([0, 9], dtype=torch.int32, device="cuda"), None, 1, 1, True)
+
+    for raised, status in (((bad_index, bad_offsets), 3), ((bad_offsets, bad_index), 3), ((bad_offsets,), 3),
+                           ((bad_index, lambda: _check(lib.gdc_selftest_wait_timeout(1000, _stream()))), 9)):
+        for f in raised:
+            f()
+        torch.cuda.synchronize()
+        assert lib.gdc_kernels_check_errors() == status
+        message = lib.gdc_last_error().decode()
+        assert ("gate index" in message) == (bad_index in raised) and ("packed offsets" in message) == (bad_offsets in raised)
+        assert ("time limit" in message) == (status == 9)
+        _done()
+
+
 def test_norm_spoiled_row_stays_alone():
     y, x, pw, pb, g, nw, nb = _norm_inputs(97, 40, 640, "layer", "layer", 1, "fp16")
     y[7, 3], x[21, 600] = math.nan, math.inf
