@@ -67,6 +67,10 @@ gdc_status gdc_packed_attention(gdc_dtype dtype, const void* q, int64_t ldq, con
   if (batch == 0 || q_rows == 0) return GDC_OK;
   if (!q || !out || !q_off || (k_rows > 0 && (!k || !v)))
     return set_error(GDC_ERR_NULL_POINTER, "gdc_packed_attention: null argument");
+  if (k_rows == 0) {  // k and v are not read, whatever they are
+    k = v = nullptr;
+    ldk = ldv = 0;
+  }
   const int64_t qw = int64_t(heads) * head_dim, kw = int64_t(kv_heads) * head_dim;
   if (ldq < qw || ldo < qw || (k_rows > 0 && (ldk < kw || ldv < kw)))
     return set_error(GDC_ERR_INVALID_INPUT, "gdc_packed_attention: a row pitch is below the row's width");
@@ -100,6 +104,7 @@ gdc_status gdc_linear_residual(gdc_dtype dtype, const void* a, int64_t lda, cons
   if (act < 0 || act > kActSilu) return set_error(GDC_ERR_INVALID_INPUT, "gdc_linear_residual: unknown activation %d", act);
   if (M == 0) return GDC_OK;
   if (!a || !w || !out) return set_error(GDC_ERR_NULL_POINTER, "gdc_linear_residual: null argument");
+  if (!residual) ldr = 0;  // the pitch of a tensor that is not there says nothing
   if (lda < K || ldw < K || ldo < N || (residual && ldr < N))
     return set_error(GDC_ERR_INVALID_INPUT, "gdc_linear_residual: a row pitch is below the row's width");
   if (lda % 8 || ldw % 8 || !aligned16(a) || !aligned16(w))
@@ -139,6 +144,9 @@ gdc_status gdc_gated_residual_norm(gdc_dtype dtype, const void* y, int64_t ldy, 
   if ((gate && gate_rows < 1) || (gate && !gate_index && gate_rows != 1 && gate_rows < rows) || (!gate && gate_index) ||
       gate_rows > kMaxRows)
     return set_error(GDC_ERR_INVALID_INPUT, "gdc_gated_residual_norm: gate_rows %lld does not fit", (long long)gate_rows);
+  if (!y) ldy = 0;  // the pitch of a tensor that is not there says nothing
+  if (!x_out) ldxo = 0;
+  if (!n_out) ldno = 0;
   if (!y && (gate || post_norm != 0))
     return set_error(GDC_ERR_INVALID_INPUT, "gdc_gated_residual_norm: a gate or post_norm needs y");
   if ((y && ldy < cols) || ldx < cols || (x_out && ldxo < cols) || (n_out && ldno < cols))

@@ -878,6 +878,29 @@ def test_norm_skips_and_reports_bad_gate_indices():
     _done()
 
 
+@pytest.mark.parametrize("pitch", [0, 3, -8, 1 << 40])
+def test_pitches_of_absent_tensors_do_not_matter(pitch):
+    lib = _lib()
+    x, w, n = _normal(43, 8, 64), _normal(44, 64, 64, std=0.1), _normal(45, 8, 64)
+    out, again, off, ws = torch.empty_like(x), torch.empty_like(x), _offsets([8]), _workspace(1, 8, 0, 1, 1, 64)
+    args = (2, x.data_ptr(), 64, w.data_ptr(), 64, None, None)
+    _check(lib.gdc_linear_residual(*args, pitch, out.data_ptr(), 64, 8, None, 64, 64, 0, _stream()))
+    _check(lib.gdc_linear_residual(*args, 0, again.data_ptr(), 64, 8, None, 64, 64, 0, _stream()))
+    _done()
+    assert torch.equal(out, again)
+    _check(lib.gdc_packed_attention(2, x.data_ptr(), 64, None, pitch, None, pitch, out.data_ptr(), 64, off.data_ptr(),
+                                    torch.zeros_like(off).data_ptr(), 1, 8, 0, 1, 1, 64, 1, 0.125, ws.data_ptr(), ws.numel(), _stream()))
+    _done()
+    assert (out == 0).all()
+    _check(lib.gdc_gated_residual_norm(2, None, pitch, x.data_ptr(), 64, 0, None, None, None, 0, None, 1.0, 2, None, None, None, pitch,
+                                       out.data_ptr(), 64, 8, None, 64, 1e-6, _stream()))
+    _check(lib.gdc_gated_residual_norm(2, n.data_ptr(), 64, x.data_ptr(), 64, 0, None, None, None, 0, None, 1.0, 0, None, None,
+                                       again.data_ptr(), 64, None, pitch, 8, None, 64, 1e-6, _stream()))
+    _done()
+    _within(out, *norm_definition(None, x, "none", None, None, None, None, 1.0, "rms", None, None, 1e-6)[1])
+    _within(again, *norm_definition(n, x, "none", None, None, None, None, 1.0, "none", None, None, 1e-6)[0])
+
+
 def test_errors_of_several_calls_are_all_named():
     """The error word holds what every call since its last reading has raised: one status, and a message that names all."""
     lib = _lib()
