@@ -301,6 +301,30 @@ def test_attention_keeps_what_is_not_seen_out(dtype, dim, bad):
         assert torch.isnan(got[150:200, :2 * dim]).all()
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("rows,n,causal", [(1, 1, True), (1, 2, True), (1, 200, False), (1, 7000, True), (40, 300, True), (500, 500, True),
+                                           (700, 900, False), (3, 4000, True)])
+@pytest.mark.parametrize("scale", [0.125, 0.75])
+def test_attention_counts_its_roundings(dtype, dim, rows, n, causal, scale):
+    """Every rounding of the computation and no more: a weight's 16-bit form (u; in fp16 at least 2^-32 of the largest weight), the
+    exponential's 2^-22, sums of n terms and a score's dim products in fp32, the exponent's own rounding, and the
+    output's u."""
+    t = DTYPES[dtype][0]
+    q, k, v = (_normal(46 + i, r, dim, dtype=t) for i, r in enumerate((rows, n, n)))
+    got = attention(q, k, v, _offsets([rows]), _offsets([n]), 1, 1, causal, scale)
+    _done()
+    see = torch.ones(rows, n, dtype=torch.bool, device="cuda")
+    see = see.tril(n - rows) if causal else see
+    w = torch.softmax((q.double() @ k.double().t() * scale).masked_fill(~see, -math.inf), -1)
+    want, reach = w @ v.double(), w @ v.double().abs()
+    mag = (q.double().abs() @ k.double().abs().t() * scale).masked_fill(~see, 0.0).amax(1, keepdim=True)
+    u, ds = torch.finfo(t).eps / 2, (dim + 8) * 2.0 ** -23 * mag
+    smallest = 2.0 ** -32 * w.amax(1, keepdim=True) * (see.double() @ v.double().abs()) if dtype == "fp16" else 0.0
+    weights = (u + 2.0 ** -22 + n * 2.0 ** -23 + 2 * ds) * (reach + want.abs()) * (1 + 2 * u) + smallest
+    _within(got, want, weights * (1 + u) + u * want.abs() + torch.finfo(t).smallest_normal * u)
+
+
 def test_attention_infinite_value_behind_many_keys():
     """64 rows that see an infinite value among 600,000 keys are computed by their definition, 32 by each of two warps one
     after the other (about 3 s); the CTA's other warps wait for them and its further items are computed."""
