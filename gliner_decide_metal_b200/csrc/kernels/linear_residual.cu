@@ -19,19 +19,21 @@
 //
 // Roles: warp 0 TMA (128-column K blocks of w and a into a ring), warp 1 MMA issue, warps 2-17
 // epilogue (TMEM lane quarter warp % 4; the four warps of a quarter take 16-column chunks in turn).
-// An epilogue warp has the residuals of its whole tile share (up to 64 rows, 64 bytes each) on
-// their way before it waits for the accumulators.
+// An epilogue warp has the residuals of its first three 16-column chunks (48 rows, 64 bytes each) on
+// their way before it waits for the accumulators, and those of three chunks ahead from then on.
 // Sums are fp32 over K in order (K split: in order inside a share, shares in rank order): the
 // same call gives the same bits.
 //
-// What bounds it, and what it reaches on a B200 (bias and residual included):
-//   8192 x 8192 x 4096 (M, N, K), GELU   the tensor cores: 390 us, 1409 TFLOP/s (a library's product
-//                      alone: 393; in power-limited runs of seconds 433 against 381)
-//   4885 x 1024 x 4096 136 of 148 SMs in one round of 512-row tiles, its start and its epilogue not
-//                      overlapped: 34 us, 1206 TFLOP/s (product alone: 30.5)
-//   4885 x 4096 x 1024, GELU   epilogues, 8 K blocks a tile long: 51 us, 803 TFLOP/s (34)
+// What bounds it, and what it reaches on a B200 (bias and residual included, fp16; 20 calls captured in a graph, their
+// tensors in turn out of 400 MB; in brackets a library's product alone the same way; "in calls": one
+// C call after another, where the clock is the power cap's):
+//   8192 x 8192 x 4096 (M, N, K), GELU   the tensor cores: 390 to 405 us, 1360 to 1410 TFLOP/s (393 to 416); in calls
+//                      440 to 450, 1220 TFLOP/s
+//   4885 x 1024 x 4096 136 of 148 SMs in one round of 288-row tiles, its start and its epilogue not
+//                      overlapped: 34 us, 1190 TFLOP/s (31); in calls 41
+//   4885 x 4096 x 1024, GELU   epilogues, 8 K blocks a tile long: 51 us, 796 TFLOP/s (35); bf16 4% less
 //   64 x 4096 x 4096, SiLU     operand tiles arriving: 14 us, 2.5 TB/s (9.7)
-//   1 x 4096 x 4096    weights streaming: 10.8 us, 3.1 TB/s (12.5)
+//   1 x 4096 x 4096    weights streaming: 10.8 us, 3.1 TB/s (11.8)
 // Tried and slower: 64-column K blocks (406 -> 575 us on the first), prefetching weights to L2 (15.4 ->
 // 17.5 us for 64 rows); polling waits and one TMA box an operand made no difference.
 #include <cuda.h>
@@ -56,7 +58,6 @@ constexpr int kThreads = 64 + 32 * kEpiWarps;
 constexpr int kMaxStages = 6;
 constexpr int kWBytes = 128 * kBK * 2;
 constexpr int kRingBytes = 225 * 1024, kSplitRing = 192 * 1024;  // (split K keeps partial sums beside the ring)
-constexpr int kSmallRing = 108 * 1024;  // leaves room for a second CTA's set-up on the SM
 constexpr int kMaxSplitBt = 64;  // split K: columns x 128 lanes x 4 bytes of partial sums, 32 KB
 constexpr int kCtrlBytes = 256;
 constexpr int kMaxSmem = kRingBytes + kCtrlBytes + 1024;
@@ -439,10 +440,13 @@ struct DeviceLimits {
   int sms = 148, clusters[4] = {148, 74, 36, 16};
 };
 
-// The form of a call: each form's estimated time in microseconds; the least wins. Measured on a
-// B200: operand tiles arrive at 95 bytes a nanosecond and SM when all SMs load, 130 when half of
-// them do (this, not the tensor cores, bounds every tile below 256 x 256); an epilogue takes 11 ns
-// a column, 9 more for a residual or a GELU; joining split K about 1.2 us.
+// The form of a call: the least of each form's estimate in microseconds wins. The constants order the forms of one
+// call as they were measured; they do not predict times. Operand tiles: 95 bytes a nanosecond and SM when all
+// SMs load, 130 when half of them do, which is what tiles that other CTAs have brought into L2 come at; weights that
+// come from HBM, as with few rows, arrive at half of that or less (all SMs: 44). An epilogue: 11 ns a column,
+// 9 more for a residual or a GELU; joining split K 1.2 us; a launch's start is left out. Estimate and time in us:
+// 1 x 4096 x 4096 4.4 and 10.8, 64 x 4096 x 4096 5.7 and 14, 4885 x 1024 x 4096 29 and 34, 4885 x 4096 x 1024 GELU 37 and
+// 51, 8192 x 8192 x 4096 GELU 317 and 390 to 405.
 Config choose(int64_t M, int N, int K, bool residual, int act, const DeviceLimits& dev) {
   Config best{false, 16, 1};
   double best_time = 1e300;
@@ -551,11 +555,12 @@ gdc_status launch_typed(const LinearResidualArgs& a, cudaStream_t stream, int* e
   const int64_t tiles = ((a.N + tile_n - 1) / tile_n) * ((a.M + c.bt - 1) / c.bt);
   const int64_t at_once = c.pair ? lim.clusters[1] : (c.split == 1 ? sms : tiles);
   const int64_t blocks = ((a.K + kBK - 1) / kBK + c.split - 1) / c.split;  // K blocks of a CTA's tile
-  // A ring holds what it can use. One that stays small leaves room for the next kernel's set-up on
-  // the SM; a tile of more K blocks than fit there uses the SM's whole shared memory.
+  // As many stages as fit and, where a CTA has one tile, as it has K blocks. (576 threads of 96 registers keep a second
+  // CTA of this kernel off the SM whatever the ring's size; only kernels of up to 10,000 registers, such as a small
+  // norm, start beside it, and chains of norms and small linears took the same time with rings of any size.)
   const bool one = tiles <= at_once;
-  const int deep = std::min(kMaxStages, (c.split > 1 ? kSplitRing : kRingBytes) / p.stage_bytes), shallow = std::min(kMaxStages, kSmallRing / p.stage_bytes);
-  p.stages = one && blocks <= shallow ? int(std::max<int64_t>(1, blocks)) : deep;
+  p.stages = std::min(kMaxStages, (c.split > 1 ? kSplitRing : kRingBytes) / p.stage_bytes);
+  if (one) p.stages = int(std::min<int64_t>(p.stages, blocks));
   p.acc_cols = (c.bt + 31) / 32 * 32;
   p.tmem_cols = 32;
   while (p.tmem_cols < (one ? 1 : 2) * p.acc_cols) p.tmem_cols *= 2;
