@@ -15,10 +15,11 @@
 // the one before it writes them, so they are not read-only for its lifetime. Rows at odd 2-byte addresses are read
 // value by value when their turn comes.
 //
-// On a B200, two norms and a gate (8 bytes a value): 16384 x 4096 RMSNorm 90 us, 6.0 TB/s (0.91 of a
-// plain copy; its instructions are next, 0.69 issued a cycle), LayerNorm 108 us (one reduction more a
-// norm); 4885 x 1024 LayerNorm 12.7 us, 3.2 TB/s (two rows a block in all: start and chain of
-// reductions); 16384 x 4095, value by value, 187 us.
+// On a B200, two norms and a gate (8 bytes a value), captured back to back: 16384 x 4096 RMSNorm 90 to 94 us, 5.7 to
+// 6.0 TB/s (0.87 to 0.91 of a plain copy; its instructions are next, 0.68 issued a cycle; 97 us one C call after another),
+// LayerNorm 107 us (one reduction more a norm); 4885 x 1024 LayerNorm 10 to 13 us, 3.2 TB/s at most from HBM (two
+// rows a block in all: start and chain of reductions); 16384 x 4095, value by value, 187 us (these variants also spill
+// up to 236 bytes a thread at 64 registers).
 #include <algorithm>
 
 #include "elem.cuh"

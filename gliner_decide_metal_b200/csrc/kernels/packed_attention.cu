@@ -48,17 +48,20 @@
 //   prompts   256 rows x 128 keys at D = 128 take the tensor cores 2048 cycles and the exponential
 //             unit 2048, but a row group's chain (scores 1250 from its weights on, maximum 500,
 //             exponentials and rounding 1450, hand-over 300) takes 3550, and two groups fill it to
-//             1.7 times the longer of the two. 8192 tokens, 32 / 8 heads of 128, causal: 456 to
-//             474 us, 1200 TFLOP/s (540 us in a power-limited run of seconds). Tried and slower: part of the
+//             1.7 times the longer of the two. 8192 tokens, 32 / 8 heads of 128, causal: 534 to 541 us, 1030 TFLOP/s,
+//             one C call after another (the power cap's clock); 459 to 516 us in short captured bursts. Tried and
+//             slower: part of the
 //             exponentials as polynomials, two threads a row, weights in halves signalled apart, two
 //             issuing warps, 64-key steps with two score buffers.
 //   D = 64    S_t is ready when its group is: waits 300, scores 300, maximum 500, exponentials 1600, 3000 in
-//             all with both groups on the exponential unit. Four prompts of 4096, 16 / 4 heads: 216 us,
-//             635 TFLOP/s (242 us with the weights over the scores).
-//   tokens    HBM: 48 tokens over 212,000 keys of 8 heads of 128: 155 us, 5.6 TB/s. One
-//             token over 8000: 18 us, of which 10 its keys and 3 the joining.
-//   short     32 sequences of 64 to 256 rows, 16 / 4 heads of 64: 29 us, of which 5 plan, 7 to 12 the
-//             first item of each CTA (its instructions are cold) and 4 to 5 each further one.
+//             all with both groups on the exponential unit. Four prompts of 4096, 16 / 4 heads: 215 to 225 us,
+//             610 to 640 TFLOP/s (242 us with the weights over the scores).
+//   tokens    HBM: 48 tokens over 212,000 keys of 8 heads of 128, captured: 154 us, 5.6 TB/s; over 196,000 more uneven
+//             ones, one C call after another, 167 us, 4.8 TB/s. One token over 8000: 18 to 25 us from one GPU
+//             to the next, of which 10 its keys and 3 the joining.
+//   short     32 sequences of 64 to 256 rows, 16 / 4 heads of 64: 30 us, of which 5 plan, 7 to 12 the
+//             first item of each CTA (its instructions are cold), 4 to 5 each further one and up to 4.7 a joining
+//             launch that finds nothing.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -131,7 +134,8 @@ PlanLayout plan_layout(int batch, int64_t q_rows, int64_t k_rows, int heads, int
   // Up to 128 sequences of one item each (tokens taken one at a time) and about 48 key tiles an SM: every CTA
   // goes over the offsets itself, which spares a launch (one token over 8000 keys 22.1 -> 18.2 us, 32 over
   // 1000 38.8 -> 35.1, 48 over 95,000 in all 92.7 -> 81.8). With more the planner's order by cost is worth it
-  // (48 over 212,000: 154 us planned, 166 so).
+  // (48 over 212,000: 154 us planned, 166 so). Measured at head size 128; at 64, whose tiles are half as large, the same
+  // limit is used unmeasured.
   const bool direct = q_rows <= per_item && batch <= 128 && (k_rows / kKeys + batch) * kv_heads <= 48 * kPlanSms;
   l.planned = l.split ? !direct : jobs > kPlanSms;
   l.chunks_cap = int(l.split ? cap / kv_heads : std::min<int64_t>(l.items_ub, INT32_MAX));
@@ -557,7 +561,8 @@ __device__ __forceinline__ int only_item(const Params& p, int b, bool report, in
 // weighs one length (the last: no splitting) by the rounds that its chunks take: 1.2 us a tile, 5.5 a round, 3
 // for joining. Measured against chunk_length: 24 tokens over 500 to 2000 keys of 8 heads of 128: 43 -> 35 us,
 // 12 over 300 to 4000: 32 -> 27 us, 32 over 1000: 35.4 both; of 64 short ones
-// the weighing costs more than it gives (22.0 -> 23.3).
+// the weighing costs more than it gives (22.0 -> 23.3). The constants are head size 128's, at 64 as well (there 24 over
+// 500 to 2000 take 30 us and 12 over 300 to 4000 26).
 __device__ __forceinline__ int weighed_length(const Params& p, int t, int longest) {
   const int lane = threadIdx.x & 31;
   const int whole = max(longest, 1), mine = lane == 31 ? whole : min(whole, (lane + 2) * (1 + longest / 48));

@@ -349,8 +349,10 @@ gdc_status gdc_linear(const uint16_t* a, const uint16_t* w, const uint16_t* bias
  * h / (heads / kv_heads):
  *   out[i, h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * q[i, h] . k[j] - max)
  * A query that sees no key gives zeros. What a query does not see never reaches its output, not
- * even where it is infinite or NaN (a row whose result is not finite is computed again by
- * one warp, which takes some 170 ns a key).
+ * even where it is infinite or NaN (a row whose result is not finite, or whose largest score passes
+ * 2.9 million, is computed again by one warp, 130 to 190 ns a key, up to 32 such rows one after
+ * the other). The p_j are rounded to the tensors' type for the product with v: a p_j is off by half a
+ * step of that type or, in fp16, by 2^-32 of the row's largest, whichever is more.
  *  q, out: q_rows rows of heads * head_dim; k, v: k_rows rows of kv_heads * head_dim; row pitches
  *  ldq, ldk, ldv, ldo in elements (q, k and v may be column blocks of one projection's output).
  *  Pointers 16-byte aligned, pitches multiples of 8. head_dim is 64 or 128, heads a multiple of
