@@ -1107,6 +1107,28 @@ def test_norm_follows_a_gate_that_the_call_before_it_writes(cols):
     assert torch.isfinite(a).all() and torch.equal(a, b)
 
 
+def test_the_three_operators_on_streams_of_their_own():
+    """Calls of every form at once on four streams, each against the same call alone."""
+    w, a = _normal(220, 1024, 512, std=0.05), _normal(221, 900, 512)
+    x, y, r = _normal(222, 900, 512), _normal(223, 900, 512), _normal(224, 900, 1024)
+    q, kv, off = _normal(225, 900, 512), _normal(226, 900, 128), _offsets([500, 400])
+    ws = _workspace(2, 900, 900, 8, 2, 64)
+    calls = [lambda out: linear(a, w, None, r, 1, out=out), lambda out: linear(a[:5], w, None, r[:5], 3, out=out),
+             lambda out: attention(q, kv, kv, off, None, 8, 2, True, out=out, ws=ws),
+             lambda out: norm(y, x, "rms", None, None, None, None, 0.5, "layer", None, None, 1e-6, x_out=out[0], n_out=out[1])]
+    make = lambda: [torch.empty_like(r), torch.empty_like(r[:5]), torch.empty_like(q), torch.empty(2, 900, 512, dtype=q.dtype, device="cuda")]  # noqa: E731
+    alone, outs, streams = make(), make(), [torch.cuda.Stream() for _ in calls]
+    for f, o in zip(calls, alone):
+        f(o)
+        torch.cuda.synchronize()
+    for _ in range(20):
+        for f, o, s in zip(calls, outs, streams):
+            with torch.cuda.stream(s):
+                f(o)
+    _done()
+    assert all(torch.equal(u, v) for u, v in zip(alone, outs))
+
+
 def test_first_use_of_a_kernel_inside_a_capture():
     """Only the first call on a device has to come before a capture; a kernel first used inside one works."""
     import subprocess
