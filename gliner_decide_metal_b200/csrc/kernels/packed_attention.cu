@@ -26,13 +26,14 @@
 // its key tiles in turn (shared_item).
 //
 // The reference m_i moves only when a row's maximum has grown by more than 2^8 (then the tile's
-// O rows are rescaled in TMEM), so most key tiles need no rescale. The weights are rounded to the tensors'
-// type: bf16 has fp32's range; in fp16 they are computed 2^7 larger (the factor is in O and in the row's sum
-// alike), so they reach up to 2^15, the range's end, and its lower end is that much further away: a weight
-// is off by 2^-11 of itself or by 2^-32 of the largest one, whichever is more. S_t(j) complete implies P_t V(j-1) complete
+// O rows are rescaled in TMEM), so most key tiles need no rescale. S_t(j) complete implies P_t V(j-1) complete
 // (one thread issues them in that order) at D = 128, so the rescale needs no wait of its own; at D = 64
-// the row warps wait for P_t V(j-1) before they write O_t or P_t. The weights are
-// rounded to the tensors' type for the second product, the row's sum is of the unrounded ones.
+// the row warps wait for P_t V(j-1) before they write O_t or P_t.
+//
+// The weights are rounded to the tensors' type for the second product, the row's sum is of the unrounded
+// ones. bf16 has fp32's range; in fp16 the weights are computed 2^7 larger (the factor is in O and in the row's
+// sum alike), so they reach up to 2^15, the range's end, and its lower end is that much further away: a
+// weight is off by 2^-11 of itself or by 2^-32 of the largest one, whichever is more.
 //
 // A value that no visible key contributes must not reach a row, but 0 * inf is NaN: a row whose
 // result is not finite is computed again from memory by one warp over exactly its visible keys
@@ -50,9 +51,8 @@
 //             exponentials and rounding 1450, hand-over 300) takes 3550, and two groups fill it to
 //             1.7 times the longer of the two. 8192 tokens, 32 / 8 heads of 128, causal: 534 to 541 us, 1030 TFLOP/s,
 //             one C call after another (the power cap's clock); 459 to 516 us in short captured bursts. Tried and
-//             slower: part of the
-//             exponentials as polynomials, two threads a row, weights in halves signalled apart, two
-//             issuing warps, 64-key steps with two score buffers.
+//             slower: part of the exponentials as polynomials, two threads a row, weights in halves signalled
+//             apart, two issuing warps, 64-key steps with two score buffers.
 //   D = 64    S_t is ready when its group is: waits 300, scores 300, maximum 500, exponentials 1600, 3000 in
 //             all with both groups on the exponential unit. Four prompts of 4096, 16 / 4 heads: 215 to 225 us,
 //             610 to 640 TFLOP/s (242 us with the weights over the scores).
