@@ -28,7 +28,7 @@
 // tensors in turn out of 400 MB; in brackets a library's product alone the same way; "in calls": one
 // C call after another, where the clock is the power cap's):
 //   8192 x 8192 x 4096 (M, N, K), GELU   the tensor cores: 390 to 405 us, 1360 to 1410 TFLOP/s (393 to 416); in calls
-//                      440 to 450, 1220 TFLOP/s
+//                      440 to 468, 1170 to 1250 TFLOP/s
 //   4885 x 1024 x 4096 136 of 148 SMs in one round of 288-row tiles, its start and its epilogue not
 //                      overlapped: 34 us, 1190 TFLOP/s (31); in calls 41
 //   4885 x 4096 x 1024, GELU   epilogues, 8 K blocks a tile long: 51 us, 796 TFLOP/s (35); bf16 4% less

@@ -57,7 +57,7 @@
 //             all with both groups on the exponential unit. Four prompts of 4096, 16 / 4 heads: 215 to 225 us,
 //             610 to 640 TFLOP/s (242 us with the weights over the scores).
 //   tokens    HBM: 48 tokens over 212,000 keys of 8 heads of 128, captured: 154 us, 5.6 TB/s; over 196,000 more uneven
-//             ones, one C call after another, 167 us, 4.8 TB/s. One token over 8000: 18 to 25 us from one GPU
+//             ones, one C call after another, 164 to 173 us, 4.6 to 4.9 TB/s. One token over 8000: 18 to 25 us from one GPU
 //             to the next, of which 10 its keys and 3 the joining.
 //   short     32 sequences of 64 to 256 rows, 16 / 4 heads of 64: 30 us, of which 5 plan, 7 to 12 the
 //             first item of each CTA (its instructions are cold), 4 to 5 each further one and up to 4.7 a joining
